@@ -300,6 +300,67 @@ int wf_grouped_fp4_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
                         const void *w_s, int64_t G, int64_t N, int64_t K, void *out,
                         void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- the operators around a layer of routed FP8 experts ------------------
+ * From the residual stream through the experts' products and back, for any
+ * number of tokens: norm + quantization, routing, dispatch lists, the grouped
+ * product, combine.  None of them keeps anything between calls. */
+
+/* RMS norm of the residual stream with an E4M3 output: the reference's
+ * RMSNorm.forward followed by act_quant (torch_ops.py:33-49), with the
+ * residual's addition in front:
+ *   h = bf16(x + residual)   (written when residual is given; h = x without)
+ *   n = h * rsqrt(mean(h^2) + eps) * weight            (32 bits)
+ *   y = bf16(n)              (written when y is given)
+ *   s = max(amax|n|, 1e-4) / 448 per 128 columns, rounded up to a power of two
+ *       with ue8m0; q = e4m3(n / s)
+ * x, residual, y, h [T, D] bf16; weight [D] f32 (or bf16 with weight_bf16);
+ * q [T, D] e4m3; s [T, D/128] of `scale_kind`.  D a multiple of 128 up to 16384.
+ * residual and h are both given or both NULL; h may be residual itself.  q
+ * comes from the 32-bit n (act_quant of y rounds once more, to bf16). */
+int wf_rms_norm_quant(const void *x, const void *residual, const void *weight, int32_t weight_bf16,
+                      int64_t T, int64_t D, float eps, int32_t ue8m0, void *q, void *s,
+                      int32_t scale_kind, void *y, void *h, void *stream);
+
+/* Expert choice from router logits [T, E] (f32, or bf16 with logits_bf16):
+ * Gate.forward (architecture.py:699-718) for any T, with a choice limited to
+ * groups, which the reference's Gate does not have.  s = score(logit), sel =
+ * s + bias (bias [E] f32 or NULL); of n_groups groups of E / n_groups
+ * neighbouring experts the topk_groups with the largest value stay (the sum of
+ * the group's two largest sel with group_top2, else its largest); the topk
+ * largest sel among them are chosen, in descending order, ties to the lower
+ * index.  out_weights [T, topk] f32 = s (divided by their sum with renorm) *
+ * route_scale; out_indices [T, topk] int64.  Scores are computed in 64 bits.  A
+ * logit or sel of -infinity masks its expert; a slot that finds no expert gets
+ * index -1 and weight 0; NaN counts as the largest value.
+ * E in 1..512, topk in 1..16, n_groups in 1..32. */
+int wf_route_topk(const void *logits, int32_t logits_bf16, const float *bias, int64_t T, int32_t E,
+                  int32_t topk, int32_t score_func, int32_t n_groups, int32_t topk_groups,
+                  int32_t group_top2, int32_t renorm, float route_scale, float *out_weights,
+                  int64_t *out_indices, void *stream);
+
+/* Rows of the experts' products from the router's choice: the where / gather
+ * of MoE.forward's expert loop (architecture.py:782-790) without its host
+ * synchronization.  indices [T, topk] int64 (or int32 with indices_64 = 0);
+ * experts [expert_offset, expert_offset + n_experts) are this rank's, a pair
+ * outside them (-1 among them) gets no row.  offsets [n_experts + 1]: expert e
+ * owns rows [offsets[e], offsets[e+1]); tokens [T * topk]: the token of each
+ * row, -1 behind the last; slots [T, topk]: the row of each pair, or -1.  Rows
+ * are in order of (expert, token, slot).  The workspace needs no initial value. */
+size_t wf_expert_dispatch_workspace_bytes(int64_t T, int32_t topk, int32_t n_experts);
+int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32_t topk,
+                       int32_t n_experts, int64_t expert_offset, int32_t *offsets, int32_t *tokens,
+                       int32_t *slots, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Back to token order: y[t] = sum over j of weights[t, j] * rows[slots[t, j]]
+ * (+ shared[t]), summed in 32 bits in ascending row order (ascending expert, as
+ * MoE.forward sums, architecture.py:785-794).  rows [R, D] bf16, slots [T, topk]
+ * int32 (a slot outside [0, R) adds nothing), weights [T, topk] f32 or NULL for
+ * 1, shared [T, D] bf16 or NULL, y [T, D] bf16, or f32 with y_f32 (a rank's
+ * partial sum).  D a multiple of 8. */
+int wf_expert_combine(const void *rows, int64_t R, const int32_t *slots, const float *weights,
+                      const void *shared, int64_t T, int32_t topk, int64_t D, void *y, int32_t y_f32,
+                      void *stream);
+
 /* Workspace bytes for the dense GEMM entry points above.  The workspace is
  * zero-filled once when allocated; its split-K counters return to zero at
  * the end of every call.  The library clears them again only when the shape

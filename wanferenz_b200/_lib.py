@@ -27,6 +27,8 @@ EXPORTS = (
     "wf_moe_sum_ranks", "wf_moe_read_error_noalloc", "wf_set_wait_limit",
     "wf_launch_count", "wf_ep_buffer_bytes", "wf_ep_alloc", "wf_ep_free", "wf_ipc_get_handle",
     "wf_ipc_open_handle", "wf_ipc_close_handle", "wf_moe_forward_ep_p2p",
+    "wf_rms_norm_quant", "wf_route_topk", "wf_expert_dispatch_workspace_bytes", "wf_expert_dispatch",
+    "wf_expert_combine",
 )
 
 
@@ -60,7 +62,7 @@ class MoeWeights(ctypes.Structure):
 
 _LIB = None
 P = ctypes.c_void_p
-I32, I64, SZ = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
+I32, I64, SZ, F32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
 
 
 def _declare(lib):
@@ -102,6 +104,11 @@ def _declare(lib):
         "wf_moe_forward_ep_p2p": (ctypes.c_int, [ctypes.POINTER(MoeConfig), ctypes.POINTER(MoeWeights), P, P,
                                                  I32, I32, I32, ctypes.POINTER(ctypes.c_void_p),
                                                  P, P, P, P, SZ, P]),
+        "wf_rms_norm_quant": (ctypes.c_int, [P, P, P, I32, I64, I64, F32, I32, P, P, I32, P, P, P]),
+        "wf_route_topk": (ctypes.c_int, [P, I32, P, I64, I32, I32, I32, I32, I32, I32, I32, F32, P, P, P]),
+        "wf_expert_dispatch_workspace_bytes": (SZ, [I64, I32, I32]),
+        "wf_expert_dispatch": (ctypes.c_int, [P, I32, I64, I32, I32, I64, P, P, P, P, SZ, P]),
+        "wf_expert_combine": (ctypes.c_int, [P, I64, P, P, P, I64, I32, I64, P, I32, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

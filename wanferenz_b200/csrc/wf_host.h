@@ -1,0 +1,29 @@
+// wf_host.h - host-side services of the library shared by its translation units
+// (defined in wf_moe.cu, which holds the error message and the launch counter).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+namespace wf {
+namespace host {
+
+// Records `msg` as the calling thread's last error and returns `code`.
+int fail(int code, const char *msg) noexcept;
+int cuda_fail(cudaError_t e, const char *what) noexcept;
+// Adds n to the count of launched kernels.
+void counted(int n = 1) noexcept;
+// SMs of the current device (0 without one).
+int sm_count() noexcept;
+// Bound of the kernels' waits on another role's progress (wf_set_wait_limit).
+long long wait_limit() noexcept;
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// cuTensorMapEncodeTiled through the runtime's driver entry point (NULL when unavailable).
+EncodeTiledFn encode_fn() noexcept;
+
+}  // namespace host
+}  // namespace wf

@@ -34,6 +34,7 @@
 #include <string>
 
 #include "../../include/wfb200.h"
+#include "wf_host.h"
 #include "wf_ptx.cuh"
 #include "wf_tc.cuh"
 
@@ -1866,10 +1867,7 @@ int ensure_attrs() {
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using wf::host::EncodeTiledFn;
 
 EncodeTiledFn encode_fn() {
     static EncodeTiledFn fn = nullptr;
@@ -2197,6 +2195,30 @@ int fill_args(const wf_moe_config *c, const wf_moe_weights *w, const void *x,
 }
 
 }  // namespace
+
+// The services of wf_host.h for the library's other translation units.
+namespace wf {
+namespace host {
+int fail(int code, const char *msg) noexcept {
+    try {
+        g_err = msg;
+    } catch (...) {  // no memory for the message: the code still says what failed
+    }
+    return code;
+}
+int cuda_fail(cudaError_t e, const char *what) noexcept {
+    try {
+        return ::cuda_fail(e, what);
+    } catch (...) {
+        return WF_E_CUDA;
+    }
+}
+void counted(int n) noexcept { ::counted(n); }
+int sm_count() noexcept { return ::sm_count(); }
+long long wait_limit() noexcept { return g_wait_limit.load(); }
+EncodeTiledFn encode_fn() noexcept { return ::encode_fn(); }
+}  // namespace host
+}  // namespace wf
 
 extern "C" {
 
