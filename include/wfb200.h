@@ -9,8 +9,8 @@
  * host thread.  No entry point allocates device memory (except the set-up
  * call wf_ep_alloc, which says so), synchronizes the
  * stream or reads device data back, except the load-time check
- * wf_fp4_scales_in_range() and the error-word reads wf_moe_read_error() and
- * wf_moe_read_error_noalloc(), which say so.
+ * wf_fp4_scales_in_range() and the error-word reads wf_moe_read_error(),
+ * wf_moe_read_error_noalloc() and wf_grouped_read_error(), which say so.
  *
  * Data formats (identical to the reference's tensors, so a reference
  * checkpoint's bytes are passed through unchanged):
@@ -350,6 +350,27 @@ size_t wf_expert_dispatch_workspace_bytes(int64_t T, int32_t topk, int32_t n_exp
 int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32_t topk,
                        int32_t n_experts, int64_t expert_offset, int32_t *offsets, int32_t *tokens,
                        int32_t *slots, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The experts' block-scaled FP8 product (fp8_gemm, torch_ops.py:93-99, per
+ * expert, as grouped_fp4_gemm is fp4_gemm per slot), for any number of rows per
+ * expert: for expert e and row r in [offsets[e], offsets[e+1])
+ *   out[r, n] = sum_k (a[i, k] * a_s[i, k/128]) * (w[e, n, k] * w_s[e, n/128, k/128])
+ * with i = rows[r], or r without a row list.  a [M, K] e4m3, a_s [M, K/128],
+ * w [E, N, K] e4m3, w_s [E, ceil(N/128), K/128], scales f32 or e8m0; offsets
+ * [E + 1] and rows [R] int32 on the device (wf_expert_dispatch's offsets and
+ * tokens), out [R, N] bf16.  Sums are in 32 bits.  offsets are clamped to
+ * [0, R], rows of out that belong to no expert are not written, and a row list
+ * entry outside [0, M) gives a row of zeros.  N a multiple of 8, K of 128, E in
+ * 1..512; a, w and out 16-byte aligned.  Device waits are bounded; one that runs
+ * out ends the call early and shows in wf_grouped_read_error. */
+int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, const void *w,
+                        const void *w_s, int32_t w_scale_kind, const int32_t *offsets,
+                        const int32_t *rows, int64_t M, int64_t R, int32_t E, int64_t N, int64_t K,
+                        void *out, void *stream);
+
+/* Synchronizes `stream`; returns 0, or WF_E_TIMEOUT when a wait of a grouped
+ * product on the current device has run out since the last read, and clears it. */
+int wf_grouped_read_error(void *stream);
 
 /* Back to token order: y[t] = sum over j of weights[t, j] * rows[slots[t, j]]
  * (+ shared[t]), summed in 32 bits in ascending row order (ascending expert, as

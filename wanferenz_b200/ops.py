@@ -16,6 +16,7 @@ way from the residual stream through the experts' products and back:
 * ``rms_norm_quant(x, weight, eps, residual)``  residual + RMS norm + E4M3 output with scales
 * ``route_topk(logits, topk, ...)``             scores, bias, groups, top-k, renormalised weights
 * ``expert_dispatch(indices, n_experts)``       the router's choice as rows in expert order
+* ``grouped_fp8_gemm(a, a_s, w, w_s, offsets, rows)``  each expert's rows times its FP8 weights
 * ``expert_combine(rows, slots, weights)``      the experts' rows back in token order
 
 These run on their tensors' device (which need not be the current one) and on its
@@ -318,6 +319,58 @@ def expert_dispatch(indices, n_experts, *, expert_offset=0):
     _run(dev, "wf_expert_dispatch", L.ptr(indices), int(indices.dtype == torch.int64), t, k, n_experts, expert_offset,
          L.ptr(offsets), L.ptr(tokens), L.ptr(slots), L.ptr(ws), need)
     return offsets, tokens, slots
+
+
+def grouped_fp8_gemm(a, a_s, w, w_s, offsets, *, rows=None, out=None):
+    """Each expert's rows times its own FP8 weights, any number of rows per expert.
+
+    For expert ``e`` and row ``r`` in ``[offsets[e], offsets[e + 1])``::
+
+        out[r] = (a[i] * a_s[i]) @ (w[e] * w_s[e])^T,   i = rows[r] (r without a row list)
+
+    ``a [M, K]`` e4m3 with ``a_s [M, K/128]``, ``w [E, N, K]`` e4m3 with ``w_s [E, ceil(N/128),
+    K/128]``, scales f32 or e8m0 (as ``act_quant`` and ``rms_norm_quant`` give them); ``offsets
+    [E + 1]`` and ``rows [R]`` int32 on the device, as ``expert_dispatch`` gives them (its
+    ``tokens`` gather a token's row for each of its experts, so no permuted copy is made).
+    Returns bf16 ``[R, N]`` (``out`` when given); rows behind ``offsets[E]`` are not written.  An
+    entry of ``rows`` outside ``[0, M)`` gives a row of zeros.  N a multiple of 8, K of 128.
+    """
+    a = _check("a", a, _E4M3)
+    dev = a.device
+    if a.dim() != 2 or w.dim() != 3 or offsets.dim() != 1:
+        raise ValueError("a must be [M, K], w [E, N, K] and offsets [E + 1]")
+    m, k = a.shape
+    e, n, _ = w.shape
+    if k == 0 or k % 128 or k > 1 << 20 or n == 0 or n % 8 or n > 1 << 20 or not 1 <= e <= 512 or e * n > 1 << 30:
+        raise ValueError(f"E {e}, N {n}, K {k}: E in 1..512, N a multiple of 8, K a multiple of 128 (at most 2^20 each)")
+    w = _check("w", w, _E4M3, dev, (e, n, k))
+    a_s = _check("a_s", a_s, _F32 + _E8M0, dev, (m, k // 128))
+    w_s = _check("w_s", w_s, _F32 + _E8M0, dev, (e, (n + 127) // 128, k // 128))
+    offsets = _check("offsets", offsets, (torch.int32,), dev, (e + 1,))
+    r = m
+    if rows is not None:
+        rows = _check("rows", rows, (torch.int32,), dev)
+        if rows.dim() != 1:
+            raise ValueError("rows must be [R]")
+        r = rows.size(0)
+    if m > 1 << 30 or r > 1 << 30:
+        raise ValueError(f"{m} rows of a, {r} rows: at most 2^30 are supported")
+    if out is None:
+        out = torch.empty(r, n, dtype=torch.bfloat16, device=dev)
+    elif _check("out", out, _BF16, dev, (r, n)) is not out:
+        raise ValueError("out must be contiguous")
+    if r:
+        if not m:
+            raise ValueError("a has no rows to take")
+        _run(dev, "wf_grouped_fp8_gemm", L.ptr(a), L.ptr(a_s), _kind(a_s), L.ptr(w), L.ptr(w_s), _kind(w_s),
+             L.ptr(offsets), L.ptr(rows), m, r, e, n, k, L.ptr(out))
+    return out
+
+
+def grouped_read_error(device=None):
+    """Raises if a device wait of ``grouped_fp8_gemm`` on ``device`` ran out since the last read (synchronizes)."""
+    with torch.cuda.device(device):
+        L.check(L.load().wf_grouped_read_error(L.stream_ptr()), "wf_grouped_read_error")
 
 
 def expert_combine(rows, slots, *, weights=None, shared=None, out_dtype=torch.bfloat16):
