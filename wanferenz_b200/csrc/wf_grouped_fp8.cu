@@ -3,9 +3,18 @@
 //   out[r, n] = sum_k (a[row(r), k] * a_s[row(r), k/128]) * (w[e, n, k] * w_s[e, n/128, k/128])
 //   for expert e and r in [offsets[e], offsets[e+1]), row(r) = rows[r] (or r)
 //
-// Weight rows are the M side of the MMA (128 per tile, exactly one block of weight
-// scales), tokens the N side: an expert's rows are cut into tiles of equal width, a
-// multiple of 16, so a few rows cost a few columns and nothing is padded to 128.
+// Weight rows are the M side of the MMA, tokens the N side: an expert's rows are cut
+// into tiles of equal width, a multiple of 32 up to 256, so a few rows cost a few
+// columns and nothing is padded to 128.  A pair of CTAs (cta_group::2) works on 256
+// weight rows: each holds 128 of them (one block of weight scales) and half of the
+// tokens in shared memory, and the products of its own 128 rows in its TMEM, so a
+// 256-wide tile moves 32 KB into each SM per 128-wide K step, half of what single
+// CTAs of 128 x 128 would.
+//
+// Scales.  With e8m0 on both sides the tensor core applies them (kind::mxf8f6f4; a
+// byte per 128 K repeated for its four 32-wide products) and sums the whole of K in
+// TMEM.  Otherwise each 128-wide K step's product goes to a fresh accumulator, and the
+// worker warps scale and add it in 32-bit registers while the next step multiplies.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -23,25 +32,32 @@ using namespace tc;
 __device__ int g_err;  // error flags of the grouped products since the last wf_grouped_read_error
 
 constexpr int MAX_E = 512;
-constexpr int NT = 128;                 // tokens per tile, at most
+constexpr int NT = 256;                                  // tokens per tile, at most
 constexpr int STAGES = 6;
-constexpr int ABYTES = 128 * 128, BBYTES = NT * 128, STAGE = ABYTES + BBYTES;
-constexpr int NACC = 4;                 // K-step accumulators in TMEM
-constexpr int SGRP = 8;                 // K steps per group of scales
-constexpr int W_PROD = 0, W_MMA = 1, W_SCALE0 = 2, W_WORK0 = 4, WORKERS = 8;
-constexpr int THREADS = 32 * (W_WORK0 + WORKERS);
-constexpr int NBAR = 2 * STAGES + 2 * NACC + 4 + 1;
-constexpr int OFF_SA = STAGES * STAGE;                   // [2][SGRP][NT] f32
-constexpr int OFF_LO = OFF_SA + 2 * SGRP * NT * 4;       // [MAX_E] first row
+constexpr int ABYTES = 128 * 128, BBYTES = NT / 2 * 128, STAGE = ABYTES + BBYTES;
+constexpr int SGRP = 8;                                  // K steps per group of scales
+constexpr int W_PROD = 0, W_MMA = 1, WORKERS = 8;
+constexpr int NBAR = 2 * STAGES + 9;
+constexpr int OFF_S = STAGES * STAGE;                    // scales: [2][SGRP][NT] f32 or [2][NT] x 8 bytes
+constexpr int OFF_LO = OFF_S + 2 * SGRP * NT * 4;        // [MAX_E] first row
 constexpr int OFF_CNT = OFF_LO + MAX_E * 4;              // [MAX_E] rows
 constexpr int OFF_T = OFF_CNT + MAX_E * 4;               // [MAX_E + 1] first token tile
-constexpr int OFF_MASK = OFF_T + (MAX_E + 4) * 4;        // [2][4] valid columns
-constexpr int OFF_BAR = OFF_MASK + 32;
+constexpr int OFF_BAR = OFF_T + (MAX_E + 4) * 4;
 constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
 static_assert(SMEM <= 232448 && OFF_BAR % 8 == 0, "shared memory");
+// TMEM columns: the tile's sums and two groups of scale factors (e8m0), or two step products (f32)
+constexpr uint32_t COL_SFA = 256, COL_SFB = 320;
+
+// e8m0: 4 scale warps (one per TMEM lane quadrant); f32: 2, and the workers' accumulators need
+// the registers of a smaller block.
+template <bool E8>
+struct Roles {
+    static constexpr int SCALE0 = E8 ? 4 : 2, SCALERS = E8 ? 4 : 2, WORK0 = SCALE0 + SCALERS;
+    static constexpr int THREADS = 32 * (WORK0 + WORKERS);
+};
 
 struct Args {
-    CUtensorMap tmW, tmA;  // weights [E*N, K], box 128 x 128; tokens [M, K], box 128 x 1 (gather)
+    CUtensorMap tmW, tmA;  // weights [E*N, K], box 128 x 128; tokens [M, K], box 128 x 16, or 128 x 1 to gather
     const void *a_s, *w_s;
     const int *offsets, *rows;
     __nv_bfloat16 *out;
@@ -49,26 +65,120 @@ struct Args {
     int M, R, E, N, K, a_f32, w_f32;
 };
 
+// ---- CTA pairs ------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's `p` in CTA 0 of the pair.
+__device__ __forceinline__ uint32_t leader_addr(const void *p) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait for a barrier that either CTA of the pair arrives on.
+__device__ __forceinline__ bool twait(uint64_t *bar, uint32_t parity, volatile int *abort, long long limit) {
+    if (try_wait_cluster(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!try_wait_cluster(bar, parity)) {
+        if (*abort) return false;
+        if (clock64() - t0 > limit) {
+            atomicOr(&g_err, kErrTimeout);
+            *abort = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
+__device__ __forceinline__ void tmem_alloc2(uint32_t *dst_smem, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Arrive on `bar` of the CTAs in `mask` once every tcgen05 operation this thread issued so far is complete.
+__device__ __forceinline__ void commit2(uint64_t *bar, uint16_t mask = 3) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(mask)
+        : "memory");
+}
+
+// Whether `v` holds in all `n` threads of the named barrier.
+__device__ __forceinline__ bool bar_all(int id, int n, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "bar.red.and.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(n), "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
+
+// ---- MMA: M = 256 over the pair, both operands K-major E4M3 ----------------
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-
-// Instruction descriptor of kind::f8f6f4: E4M3 x E4M3 -> f32, M = 128, both operands K-major.
-__device__ __forceinline__ uint32_t idesc_f8(int n) {
-    return 1u << 4 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+__device__ __forceinline__ void mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+        : "memory");
+}
+// kind::f8f6f4, f32 accumulator
+__device__ __forceinline__ uint32_t idesc_f8(int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | (256u >> 4) << 24; }
+// kind::mxf8f6f4, UE8M0 scales, byte sf_id of the scale words
+__device__ __forceinline__ uint32_t idesc_mx(int n, uint32_t sf_id) {
+    return sf_id << 4 | (uint32_t)(n >> 3) << 17 | 1u << 23 | (256u >> 7) << 27 | sf_id << 29;
 }
 
-// Four rows of the tensor map, 128 bytes each, to 512 consecutive (swizzled) bytes.
-__device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, int c0, int4 r, uint64_t *bar) {
+// ---- TMA into this CTA's memory, completion on the leader's barrier --------
+__device__ __forceinline__ void tma_load2(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+// Four rows of the tensor map, 128 bytes each, to 512 consecutive (swizzled) bytes.
+__device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, int c0, int4 r, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
         "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(smem_u32(bar))
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
         : "memory");
 }
 
@@ -84,16 +194,21 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 
+// ---- tiles -----------------------------------------------------------------
 struct Tile {
     int e, n0, r0, nrow, width;
 };
 
-// Tiles of this CTA in order: blockIdx.x, blockIdx.x + gridDim.x, ...; within an
-// expert the weight tile runs fastest.
+// Tiles of this CTA pair in order; within an expert the weight tile runs fastest.
 struct Walk {
     const int *lo, *cnt, *first;
-    int E, nn, e;
+    int E, nn, step, e;
     long long i;
     __device__ bool next(Tile &t) {
         while (e < E && i >= (long long)first[e + 1] * nn) ++e;
@@ -101,56 +216,62 @@ struct Walk {
         const int local = (int)(i - (long long)first[e] * nn);
         const int nt = first[e + 1] - first[e], c = cnt[e];
         t.e = e;
-        t.n0 = local % nn * 128;
-        t.width = ((c + nt - 1) / nt + 15) / 16 * 16;
+        t.n0 = local % nn * 256;
+        t.width = ((c + nt - 1) / nt + 31) / 32 * 32;  // cta_group::2 takes N in steps of 32
         const int j = local / nn * t.width;
         t.r0 = lo[e] + j;
         t.nrow = min(t.width, c - j);
-        i += gridDim.x;
+        i += step;
         return true;
     }
 };
 
-__device__ __forceinline__ bool twait(uint64_t *bar, uint32_t parity, volatile int *abort, long long limit) {
-    if (*abort) return false;
-    if (!wf_wait(bar, parity, &g_err, limit)) {
-        *abort = 1;
-        return false;
-    }
-    return true;
-}
 __device__ __forceinline__ float scale_at(const void *s, int f32, size_t i) {
     if (f32) return __ldg((const float *)s + i);
     const uint32_t b = __ldg((const uint8_t *)s + i);
     return b == 255 ? __uint_as_float(0x7fffffffu) : e8m0_to_f32(b);
 }
 
-__global__ void __launch_bounds__(THREADS, 1) k_grouped_f32(const __grid_constant__ Args p) {
+// The row of `a` that row r of the product reads, clamped into a; `valid` says whether it was inside.
+__device__ __forceinline__ int source_row(const Args &p, int r, bool &valid) {
+    const int s = p.rows ? __ldg(p.rows + r) : r;
+    valid = s >= 0 && s < p.M;
+    return valid ? s : 0;
+}
+
+template <bool E8>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 1)
+    k_grouped_fp8(const __grid_constant__ Args p) {
+    using L = Roles<E8>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bar = reinterpret_cast<uint64_t *>(base + OFF_BAR);
-    uint64_t *full = bar, *empty = bar + STAGES, *acc_ready = empty + STAGES, *acc_free = acc_ready + NACC;
-    uint64_t *sf_full = acc_free + NACC, *sf_empty = sf_full + 2, *fin = sf_empty + 2;
+    // full, ready-for-MMA and freed accumulators live in the leader; empty, acc_ready in both
+    uint64_t *full = bar, *empty = bar + STAGES, *acc_ready = empty + STAGES, *acc_free = acc_ready + 2;
+    uint64_t *sf_full = acc_free + 2, *sf_empty = sf_full + 2, *fin = sf_empty + 2;
     uint32_t *tmem_base = reinterpret_cast<uint32_t *>(bar + NBAR);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_base + 1);
-    float *sa = reinterpret_cast<float *>(base + OFF_SA);
     int *lo = reinterpret_cast<int *>(base + OFF_LO), *cnt = reinterpret_cast<int *>(base + OFF_CNT);
     int *first = reinterpret_cast<int *>(base + OFF_T);
-    volatile uint32_t *mask = reinterpret_cast<volatile uint32_t *>(base + OFF_MASK);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nks = p.K / 128, nn = (p.N + 127) / 128;
+    const int rank = (int)cluster_rank();
+    const int nks = p.K / 128, nn = (p.N + 255) / 256, nb = (p.N + 127) / 128;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-        for (int j = 0; j < NACC; ++j) { mbar_init(acc_ready + j, 1); mbar_init(acc_free + j, WORKERS); }
-        for (int j = 0; j < 2; ++j) { mbar_init(sf_full + j, W_WORK0 - W_SCALE0); mbar_init(sf_empty + j, WORKERS); }
+        for (int j = 0; j < 2; ++j) {
+            mbar_init(acc_ready + j, 1);
+            mbar_init(acc_free + j, 2 * WORKERS);
+            mbar_init(sf_full + j, E8 ? 2 * L::SCALERS : L::SCALERS);
+            mbar_init(sf_empty + j, E8 ? 1 : WORKERS);
+        }
         mbar_init(fin, 1);
         *abort = 0;
         fence_mbar_init();
     }
-    if (warp == W_MMA) { tmem_alloc(tmem_base, 512); tmem_relinquish(); }
+    if (warp == W_MMA) tmem_alloc2(tmem_base, 512);
     // every expert's rows, clamped to the R rows there are, and its first token tile
-    for (int e = threadIdx.x; e < p.E; e += THREADS) {
+    for (int e = threadIdx.x; e < p.E; e += L::THREADS) {
         const int a = min(max(p.offsets[e], 0), p.R), b = min(max(p.offsets[e + 1], 0), p.R);
         lo[e] = a;
         cnt[e] = max(b - a, 0);
@@ -179,158 +300,289 @@ __global__ void __launch_bounds__(THREADS, 1) k_grouped_f32(const __grid_constan
     }
     fence_before_sync();
     __syncthreads();
+    cluster_sync();
     fence_after_sync();
     const uint32_t tm = *tmem_base;
-    Walk walk{lo, cnt, first, p.E, nn, 0, (long long)blockIdx.x};
+    Walk walk{lo, cnt, first, p.E, nn, (int)(gridDim.x / 2), 0, (long long)(blockIdx.x / 2)};
     Tile t;
 
     if (warp == W_PROD) {
+        if constexpr (!E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         int gs = 0;
         bool ok = true;
         while (ok && walk.next(t)) {
-            int4 src = make_int4(0, 0, 0, 0);
-            int *s4 = reinterpret_cast<int *>(&src);
+            const int half = t.width / 2;  // this CTA's tokens of the tile
+            int src[4];
+            if (p.rows) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = t.r0 + min(4 * lane + j, t.nrow - 1);
-                s4[j] = min(max(p.rows ? __ldg(p.rows + r) : r, 0), p.M - 1);
+                for (int j = 0; j < 4; ++j) {
+                    bool valid;
+                    src[j] = source_row(p, t.r0 + min(half * rank + 4 * lane + j, t.nrow - 1), valid);
+                }
             }
             for (int ks = 0; ks < nks; ++ks, ++gs) {
                 const int st = gs % STAGES;
                 if (gs >= STAGES) ok = twait(empty + st, (gs / STAGES - 1) & 1, abort, p.limit);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 uint8_t *dst = base + st * STAGE;
+                const uint32_t fb = leader_addr(full + st);
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(full + st, ABYTES + t.width * 128);
-                    tma_load_2d(dst, &p.tmW, ks * 128, t.e * p.N + t.n0, full + st);
+                    if (rank == 0) mbar_arrive_expect_tx(full + st, 2 * (ABYTES + half * 128));
+                    tma_load2(dst, &p.tmW, ks * 128, t.e * p.N + t.n0 + 128 * rank, fb);
                 }
                 __syncwarp();
-                if (4 * lane < t.width) tma_gather4(dst + ABYTES + lane * 512, &p.tmA, ks * 128, src, full + st);
+                if (!p.rows) {
+                    if (16 * lane < half)
+                        tma_load2(dst + ABYTES + lane * 2048, &p.tmA, ks * 128, t.r0 + half * rank + 16 * lane, fb);
+                } else if (4 * lane < half)
+                    tma_gather4(dst + ABYTES + lane * 512, &p.tmA, ks * 128, make_int4(src[0], src[1], src[2], src[3]), fb);
             }
         }
-        if (*abort) {  // the copies issued must land before the CTA's memory goes
-            for (int u = max(0, gs - STAGES); u < gs; ++u) wf_wait(full + u % STAGES, (u / STAGES) & 1, &g_err);
+        // The last stages' releases arrive from the leader: none may find this CTA gone.
+        for (int u = max(0, gs - STAGES); ok && u < gs; ++u) ok = twait(empty + u % STAGES, (u / STAGES) & 1, abort, p.limit);
+        if (*abort) {
+            // The copies issued must land before the CTA's memory goes.  A pair that gave up in
+            // different places has no barrier to tell, so both wait some milliseconds.
+            const long long t0 = clock64();
+            while (clock64() - t0 < 8000000) {}
         }
     } else if (warp == W_MMA) {
-        if (lane == 0) {
-            int gs = 0;
+        if constexpr (!E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (rank == 0 && lane == 0) {
+            int gs = 0, sg = 0, ti = 0;
             bool ok = true;
-            while (ok && walk.next(t)) {
-                const uint32_t id = idesc_f8(t.width);
+            for (; ok && walk.next(t); ++ti) {
+                if (E8) ok = ti < 1 || twait(acc_free, (ti - 1) & 1, abort, p.limit);
+                if (!ok) break;
                 for (int ks = 0; ks < nks; ++ks, ++gs) {
-                    const int st = gs % STAGES, ab = gs % NACC;
-                    ok = gs < NACC || twait(acc_free + ab, (gs / NACC - 1) & 1, abort, p.limit);
+                    const int st = gs % STAGES, g = ks % SGRP, b = sg & 1, ab = gs & 1;
+                    if (E8) {
+                        if (g == 0) ok = twait(sf_full + b, (sg / 2) & 1, abort, p.limit);
+                    } else {
+                        ok = gs < 2 || twait(acc_free + ab, (gs / 2 - 1) & 1, abort, p.limit);
+                    }
                     ok = ok && twait(full + st, (gs / STAGES) & 1, abort, p.limit);
                     if (!ok) break;
                     fence_after_sync();
                     const uint64_t ad = smem_desc_sw128(base + st * STAGE), bd = smem_desc_sw128(base + st * STAGE + ABYTES);
+                    if (E8) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f8(tm + NT * ab, ad + 2 * j, bd + 2 * j, id, j != 0);
-                    commit(empty + st);
-                    commit(acc_ready + ab);
-                }
-            }
-            commit(fin);  // TMEM goes only when every MMA is done
-            wf_wait(fin, 0, &g_err);
-        }
-    } else if (warp < W_WORK0) {
-        const int i = threadIdx.x - 32 * W_SCALE0;  // this thread: tokens i and i + 64 of the tile
-        int sg = 0;
-        bool ok = true;
-        while (ok && walk.next(t)) {
-            size_t ai[2];
-            bool valid[2];
+                        for (int j = 0; j < 4; ++j)
+                            mma_mx(tm, ad + 2 * j, bd + 2 * j, idesc_mx(t.width, j), tm + COL_SFA + 4 * SGRP * b + 4 * g,
+                                   tm + COL_SFB + 8 * SGRP * b + 8 * g, (ks | j) != 0);
+                    } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = t.r0 + min(i + 64 * h, t.nrow - 1);
-                const int src = p.rows ? __ldg(p.rows + r) : r;
-                valid[h] = src >= 0 && src < p.M;
-                ai[h] = (size_t)(valid[h] ? src : 0) * nks;
-            }
-            const size_t wi = ((size_t)t.e * nn + t.n0 / 128) * nks;
-            for (int k0 = 0; k0 < nks; k0 += SGRP, ++sg) {
-                const int b = sg & 1;
-                if (sg >= 2) ok = twait(sf_empty + b, (sg / 2 - 1) & 1, abort, p.limit);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-#pragma unroll
-                for (int g = 0; g < SGRP; ++g)
-                    if (k0 + g < nks) {
-                        const float ws = scale_at(p.w_s, p.w_f32, wi + k0 + g);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            sa[(b * SGRP + g) * NT + i + 64 * h] = scale_at(p.a_s, p.a_f32, ai[h] + k0 + g) * ws;
+                        for (int j = 0; j < 4; ++j) mma_f8(tm + NT * ab, ad + 2 * j, bd + 2 * j, idesc_f8(t.width), j != 0);
                     }
+                    commit2(empty + st);
+                    if (!E8) commit2(acc_ready + ab);
+                    if (E8 && (g == SGRP - 1 || ks == nks - 1)) {
+                        commit2(sf_empty + b);
+                        ++sg;
+                    }
+                }
+                if (E8 && ok) commit2(acc_ready);
+            }
+            commit2(fin, 1);  // TMEM and the peer's operands go only when every MMA is done
+            twait(fin, 0, abort, kWaitLimitCycles);
+        }
+    } else if (warp < L::SCALE0) {
+        // (no role)
+    } else if (warp < L::WORK0) {
+        if constexpr (E8) {
+            // Scale factors into TMEM.  Every lane quadrant holds all of them, so each warp writes
+            // its own copy; the global loads are shared through shared memory.
+            uint2 *sb = reinterpret_cast<uint2 *>(base + OFF_S);
+            const int i = threadIdx.x - 32 * L::SCALE0;  // this thread loads tokens i and i + 128
+            const uint32_t lanes = tm + ((uint32_t)(32 * (warp & 3)) << 16);
+            const uint8_t *as = (const uint8_t *)p.a_s, *ws = (const uint8_t *)p.w_s;
+            const bool wide = nks % 8 == 0 && reinterpret_cast<uintptr_t>(as) % 8 == 0;
+            int sg = 0;
+            bool ok = true;
+            while (ok && walk.next(t)) {
+                size_t ai[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t m = __ballot_sync(0xffffffffu, valid[h]);
-                    if (lane == 0) mask[4 * b + i / 32 + 2 * h] = m;
+                    bool valid;
+                    ai[h] = (size_t)source_row(p, t.r0 + min(i + 128 * h, t.nrow - 1), valid) * nks;
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sf_full + b);
+                // the second CTA's rows may lie past N: any scale does, nothing of them is stored
+                const size_t wi = ((size_t)t.e * nb + min(t.n0 / 128 + rank, nb - 1)) * nks;
+                for (int k0 = 0; k0 < nks; k0 += SGRP, ++sg) {
+                    const int b = sg & 1;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (128 * h >= t.width) break;
+                        uint2 v = make_uint2(0, 0);
+                        if (wide) {
+                            v = __ldg(reinterpret_cast<const uint2 *>(as + ai[h] + k0));
+                        } else {
+#pragma unroll
+                            for (int g = 0; g < SGRP; ++g)
+                                if (k0 + g < nks) (g < 4 ? v.x : v.y) |= (uint32_t)__ldg(as + ai[h] + k0 + g) << (8 * (g & 3));
+                        }
+                        sb[b * NT + 128 * h + i] = v;
+                    }
+                    uint32_t wb[SGRP];
+#pragma unroll
+                    for (int g = 0; g < SGRP; ++g) wb[g] = k0 + g < nks ? __ldg(ws + wi + k0 + g) * 0x01010101u : 0u;
+                    if (sg >= 2) ok = twait(sf_empty + b, (sg / 2 - 1) & 1, abort, p.limit);
+                    ok = bar_all(1, 32 * L::SCALERS, ok);  // the warps agree: none is left at a barrier
+                    if (!ok) break;
+                    fence_after_sync();
+                    uint2 v[NT / 32];
+#pragma unroll
+                    for (int c = 0; c < NT / 32; ++c) v[c] = sb[b * NT + 32 * c + lane];
+#pragma unroll
+                    for (int g = 0; g < SGRP; ++g) {
+                        if (k0 + g >= nks) break;
+                        uint32_t f[NT / 32];
+#pragma unroll
+                        for (int c = 0; c < NT / 32; ++c) f[c] = __byte_perm(g < 4 ? v[c].x : v[c].y, 0, 0x1111 * (g & 3));
+                        tmem_st8(lanes + COL_SFB + 8 * (SGRP * b + g), f);
+                        tmem_st4(lanes + COL_SFA + 4 * (SGRP * b + g), wb[g], wb[g], wb[g], wb[g]);
+                    }
+                    tmem_wait_st();
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) arrive_at(leader_addr(sf_full + b));
+                }
+            }
+            for (int u = max(0, sg - 2); ok && u < sg; ++u) ok = twait(sf_empty + (u & 1), (u / 2) & 1, abort, p.limit);
+        } else {
+            // token scale x weight scale of each K step into shared memory
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+            float *sa = reinterpret_cast<float *>(base + OFF_S);
+            const int i = threadIdx.x - 32 * L::SCALE0;  // this thread: tokens i, i + 64, ...
+            int sg = 0;
+            bool ok = true;
+            while (ok && walk.next(t)) {
+                size_t ai[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    bool valid;
+                    ai[h] = (size_t)source_row(p, t.r0 + min(i + 64 * h, t.nrow - 1), valid) * nks;
+                }
+                const size_t wi = ((size_t)t.e * nb + min(t.n0 / 128 + rank, nb - 1)) * nks;
+                for (int k0 = 0; k0 < nks; k0 += SGRP, ++sg) {
+                    const int b = sg & 1;
+                    if (sg >= 2) ok = twait(sf_empty + b, (sg / 2 - 1) & 1, abort, p.limit);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    // all loads of the group before the first use: one trip to memory, not one per step
+                    float w[SGRP], v[4][SGRP];
+#pragma unroll
+                    for (int g = 0; g < SGRP; ++g) {
+                        const int k = min(k0 + g, nks - 1);
+                        w[g] = scale_at(p.w_s, p.w_f32, wi + k);
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) v[h][g] = 64 * h < t.width ? scale_at(p.a_s, p.a_f32, ai[h] + k) : 0.f;
+                    }
+#pragma unroll
+                    for (int g = 0; g < SGRP; ++g)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+                            if (64 * h < t.width) sa[(b * SGRP + g) * NT + i + 64 * h] = v[h][g] * w[g];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sf_full + b);
+                }
             }
         }
     } else {
-        const int q = warp & 3, half = (warp - W_WORK0) >> 2;
-        const uint32_t col = tm + ((uint32_t)(32 * q) << 16) + 64 * half;
-        int gs = 0, sg = 0;
+        // workers: warp (q, half) takes the 32 weight rows of TMEM lane quadrant q and 128 of the
+        // tile's tokens
+        if constexpr (!E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int q = warp & 3, half = (warp - L::WORK0) >> 2;
+        const uint32_t col = tm + ((uint32_t)(32 * q) << 16) + 128 * half;
+        const float *sa = reinterpret_cast<const float *>(base + OFF_S) + 128 * half;
+        int gs = 0, sg = 0, ti = 0;
         bool ok = true;
-        while (ok && walk.next(t)) {
-            float acc[64];
+        for (; ok && walk.next(t); ++ti) {
+            const int mine = min(t.nrow - 128 * half, 128);  // tokens of this warp that are stored
+            uint32_t keep[4];  // those whose row of `a` exists; the others' results are zero
 #pragma unroll
-            for (int j = 0; j < 64; ++j) acc[j] = 0.f;
-            uint32_t m[2] = {0, 0};
-            for (int ks = 0; ks < nks; ++ks, ++gs) {
-                const int g = ks % SGRP, b = sg & 1, ab = gs % NACC;
-                if (g == 0) {
-                    ok = twait(sf_full + b, (sg / 2) & 1, abort, p.limit);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    m[0] = mask[4 * b + 2 * half];
-                    m[1] = mask[4 * b + 2 * half + 1];
-                }
-                ok = twait(acc_ready + ab, (gs / NACC) & 1, abort, p.limit);
+            for (int c = 0; c < 4; ++c) {
+                bool valid = true;
+                if (32 * c + lane < mine) source_row(p, t.r0 + 128 * half + 32 * c + lane, valid);
+                keep[c] = __ballot_sync(0xffffffffu, valid);
+            }
+            const int n = t.n0 + 128 * rank + 32 * q + lane;
+            __nv_bfloat16 *o = p.out + (size_t)(t.r0 + 128 * half) * p.N + n;
+            if constexpr (E8) {
+                ok = twait(acc_ready, ti & 1, abort, p.limit);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 fence_after_sync();
-                const float *s = sa + (b * SGRP + g) * NT + 64 * half;
+                __nv_bfloat162 y[64];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    if (64 * half + 32 * c < t.width) {
-                        uint32_t v[32];
-                        tmem_ld32(col + NT * ab + 32 * c, v);
-                        tmem_wait_ld();
+                for (int c = 0; c < 4; ++c) {
+                    if (128 * half + 32 * c >= t.width) break;
+                    uint32_t v[32];
+                    tmem_ld32(col + 32 * c, v);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 f = *reinterpret_cast<const float4 *>(s + 32 * c + j);
-                            acc[32 * c + j] += f.x * __uint_as_float(v[j]);
-                            acc[32 * c + j + 1] += f.y * __uint_as_float(v[j + 1]);
-                            acc[32 * c + j + 2] += f.z * __uint_as_float(v[j + 2]);
-                            acc[32 * c + j + 3] += f.w * __uint_as_float(v[j + 3]);
-                        }
-                    }
+                    for (int j = 0; j < 16; ++j)
+                        y[16 * c + j] = __floats2bfloat162_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
                 }
                 fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_free + ab);
-                if (g == SGRP - 1 || ks == nks - 1) {
-                    if (lane == 0) mbar_arrive(sf_empty + b);
-                    ++sg;
-                }
-            }
-            if (!ok) break;
-            const int n = t.n0 + 32 * q + lane;
-            if (n < p.N) {
-                __nv_bfloat16 *o = p.out + (size_t)(t.r0 + 64 * half) * p.N + n;
+                if (lane == 0) arrive_at(leader_addr(acc_free));
+                if (n < p.N) {
 #pragma unroll
-                for (int j = 0; j < 64; ++j)
-                    if (64 * half + j < t.nrow)
-                        o[(size_t)j * p.N] = __float2bfloat16_rn(m[j / 32] >> (j % 32) & 1 ? acc[j] : 0.f);
+                    for (int j = 0; j < 128; ++j)
+                        if (j < mine)
+                            o[(size_t)j * p.N] = !(keep[j / 32] >> (j % 32) & 1) ? __float2bfloat16_rn(0.f)
+                                                 : j & 1                        ? __high2bfloat16(y[j / 2])
+                                                                                : __low2bfloat16(y[j / 2]);
+                }
+            } else {
+                float acc[128];
+#pragma unroll
+                for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+                for (int ks = 0; ks < nks; ++ks, ++gs) {
+                    const int g = ks % SGRP, b = sg & 1, ab = gs & 1;
+                    if (g == 0) ok = twait(sf_full + b, (sg / 2) & 1, abort, p.limit);
+                    ok = ok && twait(acc_ready + ab, (gs / 2) & 1, abort, p.limit);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    fence_after_sync();
+                    const float *s = sa + (b * SGRP + g) * NT;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (128 * half + 32 * c < t.width) {
+                            uint32_t v[32];
+                            tmem_ld32(col + NT * ab + 32 * c, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const float4 f = *reinterpret_cast<const float4 *>(s + 32 * c + j);
+                                acc[32 * c + j] += f.x * __uint_as_float(v[j]);
+                                acc[32 * c + j + 1] += f.y * __uint_as_float(v[j + 1]);
+                                acc[32 * c + j + 2] += f.z * __uint_as_float(v[j + 2]);
+                                acc[32 * c + j + 3] += f.w * __uint_as_float(v[j + 3]);
+                            }
+                        }
+                    }
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        arrive_at(leader_addr(acc_free + ab));
+                        if (g == SGRP - 1 || ks == nks - 1) mbar_arrive(sf_empty + b);
+                    }
+                    if (g == SGRP - 1 || ks == nks - 1) ++sg;
+                }
+                if (!ok) break;
+                if (n < p.N) {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (j < mine) o[(size_t)j * p.N] = __float2bfloat16_rn(keep[j / 32] >> (j % 32) & 1 ? acc[j] : 0.f);
+                }
             }
         }
     }
     fence_before_sync();
     __syncthreads();
+    cluster_sync();  // the pair's operands, barriers and TMEM are read by both
     if (warp == W_MMA) {
         fence_after_sync();
-        tmem_dealloc(tm, 512);
+        tmem_dealloc2(tm, 512);
     }
 }
 
@@ -369,7 +621,7 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
         return fail(WF_E_ARG, "a, w and out must be 16-byte aligned, f32 scales and row lists 4-byte");
     wf::grp::Args p;
     int rc = wf::grp::tensor_map(&p.tmW, w, (uint64_t)E * N, K, 128);
-    if (!rc) rc = wf::grp::tensor_map(&p.tmA, a, M, K, 1);
+    if (!rc) rc = wf::grp::tensor_map(&p.tmA, a, M, K, rows ? 1 : 16);
     if (rc) return rc;
     p.a_s = a_s; p.w_s = w_s; p.offsets = offsets; p.rows = rows; p.out = (__nv_bfloat16 *)out;
     p.limit = wf::host::wait_limit();
@@ -377,10 +629,15 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
     p.a_f32 = a_scale_kind == WF_SCALE_F32; p.w_f32 = w_scale_kind == WF_SCALE_F32;
     const int sms = wf::host::sm_count();
     if (sms <= 0) return fail(WF_E_CUDA, "no CUDA device");
-    cudaError_t e = cudaFuncSetAttribute(wf::grp::k_grouped_f32, cudaFuncAttributeMaxDynamicSharedMemorySize, wf::grp::SMEM);
+    const int64_t tiles = (R / wf::grp::NT + (E < R ? E : R)) * ((N + 255) / 256);
+    const unsigned grid = 2 * (unsigned)(tiles < sms / 2 ? tiles : sms / 2);
+    const bool e8 = !p.a_f32 && !p.w_f32;
+    const void *k = e8 ? (const void *)wf::grp::k_grouped_fp8<true> : (const void *)wf::grp::k_grouped_fp8<false>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, wf::grp::SMEM);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(grouped_fp8_gemm)");
-    const int64_t tiles = (R / wf::grp::NT + (E < R ? E : R)) * ((N + 127) / 128);
-    wf::grp::k_grouped_f32<<<(unsigned)(tiles < sms ? tiles : sms), wf::grp::THREADS, wf::grp::SMEM, (cudaStream_t)stream>>>(p);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (e8) wf::grp::k_grouped_fp8<true><<<grid, wf::grp::Roles<true>::THREADS, wf::grp::SMEM, st>>>(p);
+    else wf::grp::k_grouped_fp8<false><<<grid, wf::grp::Roles<false>::THREADS, wf::grp::SMEM, st>>>(p);
     wf::host::counted();
     e = cudaGetLastError();
     return e == cudaSuccess ? WF_OK : cuda_fail(e, "grouped_fp8_gemm launch");
