@@ -366,7 +366,12 @@ int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32
 int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, const void *w,
                         const void *w_s, int32_t w_scale_kind, const int32_t *offsets,
                         const int32_t *rows, int64_t M, int64_t R, int32_t E, int64_t N, int64_t K,
-                        void *out, void *stream);
+                        void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace for the call above (no initial value needed; 16-byte aligned): the listed
+ * rows in expert order, R * K, when a row list has many rows per expert, else 0 (then the
+ * workspace may be NULL).  row_list: whether rows is given. */
+size_t wf_grouped_fp8_workspace_bytes(int32_t row_list, int64_t R, int32_t E, int64_t K);
 
 /* Synchronizes `stream`; returns 0, or WF_E_TIMEOUT when a wait of a grouped
  * product on the current device has run out since the last read, and clears it. */

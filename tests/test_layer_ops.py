@@ -92,8 +92,8 @@ def test_operators_take_cuda_tensors_only():
         ops.expert_combine(x, torch.zeros(2, 1, dtype=torch.int32))
 
 
-def _grouped(a=P, a_s=P, ak=F32, w=P, w_s=P, wk=F32, off=P, rows=P, M=8, R=12, E=4, N=256, K=256, out=P):
-    return L.load().wf_grouped_fp8_gemm(a, a_s, ak, w, w_s, wk, off, rows, M, R, E, N, K, out, None)
+def _grouped(a=P, a_s=P, ak=F32, w=P, w_s=P, wk=F32, off=P, rows=P, M=8, R=12, E=4, N=256, K=256, out=P, ws=None, n=0):
+    return L.load().wf_grouped_fp8_gemm(a, a_s, ak, w, w_s, wk, off, rows, M, R, E, N, K, out, ws, n, None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -102,6 +102,7 @@ def _grouped(a=P, a_s=P, ak=F32, w=P, w_s=P, wk=F32, off=P, rows=P, M=8, R=12, E
     (dict(M=0), L.WF_E_SHAPE), (dict(R=0), L.WF_E_SHAPE), (dict(R=1 << 31), L.WF_E_SHAPE), (dict(rows=None), L.WF_E_SHAPE),
     (dict(E=0), L.WF_E_SHAPE), (dict(E=513), L.WF_E_SHAPE), (dict(N=0), L.WF_E_SHAPE), (dict(N=12), L.WF_E_SHAPE),
     (dict(E=512, N=1 << 22), L.WF_E_SHAPE), (dict(K=0), L.WF_E_SHAPE), (dict(K=192), L.WF_E_SHAPE),
+    (dict(R=1024), L.WF_E_ARG), (dict(R=1024, ws=P, n=1024 * 256 - 1), L.WF_E_ARG), (dict(R=1024, ws=ODD, n=1 << 20), L.WF_E_ARG),
     (dict(a=ctypes.c_void_p(4104)), L.WF_E_ARG), (dict(w=ctypes.c_void_p(4104)), L.WF_E_ARG),
     (dict(out=ctypes.c_void_p(4104)), L.WF_E_ARG), (dict(a_s=ODD), L.WF_E_ARG), (dict(rows=ODD), L.WF_E_ARG)])
 def test_grouped_fp8_gemm_refuses(kw, code):

@@ -28,7 +28,7 @@ EXPORTS = (
     "wf_launch_count", "wf_ep_buffer_bytes", "wf_ep_alloc", "wf_ep_free", "wf_ipc_get_handle",
     "wf_ipc_open_handle", "wf_ipc_close_handle", "wf_moe_forward_ep_p2p",
     "wf_rms_norm_quant", "wf_route_topk", "wf_expert_dispatch_workspace_bytes", "wf_expert_dispatch",
-    "wf_expert_combine", "wf_grouped_fp8_gemm", "wf_grouped_read_error",
+    "wf_expert_combine", "wf_grouped_fp8_gemm", "wf_grouped_fp8_workspace_bytes", "wf_grouped_read_error",
 )
 
 
@@ -108,7 +108,8 @@ def _declare(lib):
         "wf_route_topk": (ctypes.c_int, [P, I32, P, I64, I32, I32, I32, I32, I32, I32, I32, F32, P, P, P]),
         "wf_expert_dispatch_workspace_bytes": (SZ, [I64, I32, I32]),
         "wf_expert_dispatch": (ctypes.c_int, [P, I32, I64, I32, I32, I64, P, P, P, P, SZ, P]),
-        "wf_grouped_fp8_gemm": (ctypes.c_int, [P, P, I32, P, P, I32, P, P, I64, I64, I32, I64, I64, P, P]),
+        "wf_grouped_fp8_workspace_bytes": (SZ, [I32, I64, I32, I64]),
+        "wf_grouped_fp8_gemm": (ctypes.c_int, [P, P, I32, P, P, I32, P, P, I64, I64, I32, I64, I64, P, P, SZ, P]),
         "wf_grouped_read_error": (ctypes.c_int, [P]),
         "wf_expert_combine": (ctypes.c_int, [P, I64, P, P, P, I64, I32, I64, P, I32, P]),
     }

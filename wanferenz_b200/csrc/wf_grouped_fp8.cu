@@ -36,6 +36,7 @@ constexpr int NT = 256;                                  // tokens per tile, at 
 constexpr int STAGES = 6;
 constexpr int ABYTES = 128 * 128, BBYTES = NT / 2 * 128, STAGE = ABYTES + BBYTES;
 constexpr int SGRP = 8;                                  // K steps per group of scales
+constexpr int GATHER_ROWS = 64;                          // rows per expert up to which row lists are gathered in place
 constexpr int W_PROD = 0, W_MMA = 1, WORKERS = 8;
 constexpr int NBAR = 2 * STAGES + 9;
 constexpr int OFF_S = STAGES * STAGE;                    // scales: [2][SGRP][NT] f32 or [2][NT] x 8 bytes
@@ -57,12 +58,14 @@ struct Roles {
 };
 
 struct Args {
-    CUtensorMap tmW, tmA;  // weights [E*N, K], box 128 x 128; tokens [M, K], box 128 x 16, or 128 x 1 to gather
+    CUtensorMap tmW;     // weights [E*N, K], box 128 x 128
+    CUtensorMap tmA[4];  // rows [M, K], boxes of 128, 64, 32 and 16 rows; the first of one row to gather
     const void *a_s, *w_s;
     const int *offsets, *rows;
     __nv_bfloat16 *out;
     long long limit;
     int M, R, E, N, K, a_f32, w_f32;
+    int gather;          // the tensor map's rows are those of `rows`, else the product's own
 };
 
 // ---- CTA pairs ------------------------------------------------------------
@@ -80,25 +83,18 @@ __device__ __forceinline__ uint32_t leader_addr(const void *p) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
     return r;
 }
+// The pair's barriers hand over TMEM (ordered by the tcgen05 fences) and copies of the
+// async proxy, no ordinary memory, so arrivals and waits keep the default CTA scope:
+// cluster scope would flush stores on every arrival and drop the L1 on every wait
+// (measured: over 1000 cycles of each K step's hand-over).
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait for a barrier that either CTA of the pair arrives on.
+// Bounded wait; a wait that runs out sets the error flag and tells the CTA's other roles.
 __device__ __forceinline__ bool twait(uint64_t *bar, uint32_t parity, volatile int *abort, long long limit) {
-    if (try_wait_cluster(bar, parity)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
-    while (!try_wait_cluster(bar, parity)) {
+    while (!mbar_try_wait(bar, parity)) {
         if (*abort) return false;
         if (clock64() - t0 > limit) {
             atomicOr(&g_err, kErrTimeout);
@@ -137,6 +133,16 @@ __device__ __forceinline__ bool bar_all(int id, int n, bool v) {
         : "=r"(r)
         : "r"(id), "r"(n), "r"((uint32_t)v)
         : "memory");
+    return r != 0;
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
     return r != 0;
 }
 
@@ -253,7 +259,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_base + 1);
     int *lo = reinterpret_cast<int *>(base + OFF_LO), *cnt = reinterpret_cast<int *>(base + OFF_CNT);
     int *first = reinterpret_cast<int *>(base + OFF_T);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int nks = p.K / 128, nn = (p.N + 255) / 256, nb = (p.N + 127) / 128;
 
@@ -313,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
         while (ok && walk.next(t)) {
             const int half = t.width / 2;  // this CTA's tokens of the tile
             int src[4];
-            if (p.rows) {
+            if (p.gather) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     bool valid;
@@ -331,11 +337,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
                     tma_load2(dst, &p.tmW, ks * 128, t.e * p.N + t.n0 + 128 * rank, fb);
                 }
                 __syncwarp();
-                if (!p.rows) {
-                    if (16 * lane < half)
-                        tma_load2(dst + ABYTES + lane * 2048, &p.tmA, ks * 128, t.r0 + half * rank + 16 * lane, fb);
-                } else if (4 * lane < half)
-                    tma_gather4(dst + ABYTES + lane * 512, &p.tmA, ks * 128, make_int4(src[0], src[1], src[2], src[3]), fb);
+                if (p.gather) {
+                    if (4 * lane < half)
+                        tma_gather4(dst + ABYTES + lane * 512, &p.tmA[0], ks * 128, make_int4(src[0], src[1], src[2], src[3]), fb);
+                } else if (lane < 4 && half & 128 >> lane) {
+                    // half as a sum of boxes, one a lane: a copy costs the TMA unit about as much
+                    // whatever its height (boxes of 16 rows alone: 2091 against 3050 TFLOP/s for one
+                    // expert of 16384 rows, 4096 x 4096)
+                    const int at = half & ~(0xff >> lane);
+                    tma_load2(dst + ABYTES + at * 128, &p.tmA[lane], ks * 128, t.r0 + half * rank + at, fb);
+                }
             }
         }
         // The last stages' releases arrive from the leader: none may find this CTA gone.
@@ -348,42 +359,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
         }
     } else if (warp == W_MMA) {
         if constexpr (!E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (rank == 0 && lane == 0) {
-            int gs = 0, sg = 0, ti = 0;
+        // The whole warp walks the loop and one elected lane issues, so that descriptors stay in
+        // uniform registers (a loop run by one lane alone moves every operand there by itself:
+        // 850 cycles per K step, more than its product takes).
+        if (rank == 0) {
+            const bool leader = elect_one();
+            const uint64_t ad0 = smem_desc_sw128(base), bd0 = smem_desc_sw128(base + ABYTES);
+            int st = 0, gs = 0, sg = 0, ti = 0;
+            uint32_t phase = 0;
             bool ok = true;
             for (; ok && walk.next(t); ++ti) {
+                const int width = __shfl_sync(0xffffffffu, t.width, 0);
                 if (E8) ok = ti < 1 || twait(acc_free, (ti - 1) & 1, abort, p.limit);
-                if (!ok) break;
+                if (!__all_sync(0xffffffffu, ok)) break;
                 for (int ks = 0; ks < nks; ++ks, ++gs) {
-                    const int st = gs % STAGES, g = ks % SGRP, b = sg & 1, ab = gs & 1;
+                    const int g = ks % SGRP, b = sg & 1, ab = gs & 1;
                     if (E8) {
                         if (g == 0) ok = twait(sf_full + b, (sg / 2) & 1, abort, p.limit);
                     } else {
                         ok = gs < 2 || twait(acc_free + ab, (gs / 2 - 1) & 1, abort, p.limit);
                     }
-                    ok = ok && twait(full + st, (gs / STAGES) & 1, abort, p.limit);
-                    if (!ok) break;
+                    ok = ok && twait(full + st, phase, abort, p.limit);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     fence_after_sync();
-                    const uint64_t ad = smem_desc_sw128(base + st * STAGE), bd = smem_desc_sw128(base + st * STAGE + ABYTES);
-                    if (E8) {
+                    if (leader) {
+                        const uint64_t ad = ad0 + st * (STAGE / 16), bd = bd0 + st * (STAGE / 16);
+                        if (E8) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            mma_mx(tm, ad + 2 * j, bd + 2 * j, idesc_mx(t.width, j), tm + COL_SFA + 4 * SGRP * b + 4 * g,
-                                   tm + COL_SFB + 8 * SGRP * b + 8 * g, (ks | j) != 0);
-                    } else {
+                            for (int j = 0; j < 4; ++j)
+                                mma_mx(tm, ad + 2 * j, bd + 2 * j, idesc_mx(width, j), tm + COL_SFA + 4 * (SGRP * b + g),
+                                       tm + COL_SFB + 8 * (SGRP * b + g), (ks | j) != 0);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_f8(tm + NT * ab, ad + 2 * j, bd + 2 * j, idesc_f8(t.width), j != 0);
+                            for (int j = 0; j < 4; ++j) mma_f8(tm + NT * ab, ad + 2 * j, bd + 2 * j, idesc_f8(width), j != 0);
+                        }
+                        commit2(empty + st);
+                        if (!E8) commit2(acc_ready + ab);
+                        if (E8 && (g == SGRP - 1 || ks == nks - 1)) commit2(sf_empty + b);
                     }
-                    commit2(empty + st);
-                    if (!E8) commit2(acc_ready + ab);
-                    if (E8 && (g == SGRP - 1 || ks == nks - 1)) {
-                        commit2(sf_empty + b);
-                        ++sg;
-                    }
+                    __syncwarp();
+                    if (g == SGRP - 1 || ks == nks - 1) ++sg;
+                    if (++st == STAGES) { st = 0; phase ^= 1; }
                 }
-                if (E8 && ok) commit2(acc_ready);
+                if (E8 && ok && leader) commit2(acc_ready);
+                __syncwarp();
             }
-            commit2(fin, 1);  // TMEM and the peer's operands go only when every MMA is done
+            if (leader) commit2(fin, 1);  // TMEM and the peer's operands go only when every MMA is done
             twait(fin, 0, abort, kWaitLimitCycles);
         }
     } else if (warp < L::SCALE0) {
@@ -586,6 +607,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
     }
 }
 
+// The listed rows of a in the product's order (rows that do not exist: row 0, their results are zeroed).
+constexpr int PACK_STEP = 4 * 256;
+__global__ void __launch_bounds__(256) k_pack_rows(const uint4 *a, const int *rows, const int *offsets, uint4 *out, int E,
+                                                   int M, int R, int chunks) {
+    // rows behind the last expert's are left out; the offsets need not rise
+    int end = 0;
+    for (int e = threadIdx.x; e <= E; e += 256) end = max(end, __ldg(offsets + e));
+    __shared__ int ends[8];
+    end = __reduce_max_sync(0xffffffffu, end);
+    if (threadIdx.x % 32 == 0) ends[threadIdx.x / 32] = end;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) end = max(end, ends[w]);
+    const long long n = (long long)min(end, R) * chunks;
+    for (long long i0 = (long long)blockIdx.x * PACK_STEP + threadIdx.x; i0 < n; i0 += (long long)gridDim.x * PACK_STEP) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const long long i = min(i0 + 256 * j, n - 1);
+            const int r = (int)(i / chunks), s = __ldg(rows + r);
+            v[j] = __ldg(a + (size_t)(s >= 0 && s < M ? s : 0) * chunks + (i - (long long)r * chunks));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + 256 * j < n) out[i0 + 256 * j] = v[j];
+    }
+}
+
 int tensor_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t K, uint32_t box_rows) {
     host::EncodeTiledFn enc = host::encode_fn();
     if (!enc) return host::fail(WF_E_CUDA, "cuTensorMapEncodeTiled unavailable");
@@ -606,9 +655,15 @@ using wf::host::fail;
 
 extern "C" {
 
+size_t wf_grouped_fp8_workspace_bytes(int32_t row_list, int64_t R, int32_t E, int64_t K) {
+    if (R <= 0 || R > (1 << 30) || E <= 0 || E > wf::grp::MAX_E || K <= 0 || K > (1 << 20)) return 0;
+    return row_list && R > (int64_t)E * wf::grp::GATHER_ROWS ? (size_t)R * K : 0;
+}
+
 int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, const void *w, const void *w_s,
                         int32_t w_scale_kind, const int32_t *offsets, const int32_t *rows, int64_t M, int64_t R,
-                        int32_t E, int64_t N, int64_t K, void *out, void *stream) {
+                        int32_t E, int64_t N, int64_t K, void *out, void *workspace,
+                        size_t workspace_bytes, void *stream) {
     if (!a || !a_s || !w || !w_s || !offsets || !out) return fail(WF_E_ARG, "null pointer");
     if (a_scale_kind < 0 || a_scale_kind > 1 || w_scale_kind < 0 || w_scale_kind > 1) return fail(WF_E_DTYPE, "bad scale kind");
     if (M <= 0 || M > (1 << 30) || R <= 0 || R > (1 << 30)) return fail(WF_E_SHAPE, "M and R must be in 1..2^30");
@@ -620,8 +675,23 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
         (a_scale_kind == WF_SCALE_F32 && (uintptr_t)a_s % 4) || (w_scale_kind == WF_SCALE_F32 && (uintptr_t)w_s % 4))
         return fail(WF_E_ARG, "a, w and out must be 16-byte aligned, f32 scales and row lists 4-byte");
     wf::grp::Args p;
+    // Many rows per expert: a copy of the listed rows in expert order, then whole boxes of it.  Few:
+    // four rows a copy straight from a.  The TMA unit takes about 80 cycles for a four-row copy, so up
+    // to 32 rows of a CTA (a tile of 64) hide behind the 128 weight rows of a K step (about 700 cycles of
+    // its share of HBM), and 128 take four times as long as their product.
+    const bool pack = rows && R > (int64_t)E * wf::grp::GATHER_ROWS;
+    if (pack) {
+        if (!workspace || workspace_bytes < (size_t)R * K) return fail(WF_E_ARG, "workspace too small (see wf_grouped_fp8_workspace_bytes)");
+        if ((uintptr_t)workspace % 16) return fail(WF_E_ARG, "workspace must be 16-byte aligned");
+    }
+    p.gather = rows && !pack;
     int rc = wf::grp::tensor_map(&p.tmW, w, (uint64_t)E * N, K, 128);
-    if (!rc) rc = wf::grp::tensor_map(&p.tmA, a, M, K, rows ? 1 : 16);
+    if (p.gather) {
+        if (!rc) rc = wf::grp::tensor_map(&p.tmA[0], a, M, K, 1);
+        for (int j = 1; j < 4; ++j) p.tmA[j] = p.tmA[0];
+    } else {
+        for (int j = 0; j < 4 && !rc; ++j) rc = wf::grp::tensor_map(&p.tmA[j], pack ? workspace : a, pack ? R : M, K, 128 >> j);
+    }
     if (rc) return rc;
     p.a_s = a_s; p.w_s = w_s; p.offsets = offsets; p.rows = rows; p.out = (__nv_bfloat16 *)out;
     p.limit = wf::host::wait_limit();
@@ -636,6 +706,12 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, wf::grp::SMEM);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(grouped_fp8_gemm)");
     cudaStream_t st = (cudaStream_t)stream;
+    if (pack) {
+        const int64_t steps = R * (K / 16) / wf::grp::PACK_STEP + 1;
+        wf::grp::k_pack_rows<<<(unsigned)(steps < 8 * sms ? steps : 8 * sms), 256, 0, st>>>(
+            (const uint4 *)a, rows, offsets, (uint4 *)workspace, E, (int)M, (int)R, (int)(K / 16));
+        wf::host::counted();
+    }
     if (e8) wf::grp::k_grouped_fp8<true><<<grid, wf::grp::Roles<true>::THREADS, wf::grp::SMEM, st>>>(p);
     else wf::grp::k_grouped_fp8<false><<<grid, wf::grp::Roles<false>::THREADS, wf::grp::SMEM, st>>>(p);
     wf::host::counted();

@@ -362,8 +362,10 @@ def grouped_fp8_gemm(a, a_s, w, w_s, offsets, *, rows=None, out=None):
     if r:
         if not m:
             raise ValueError("a has no rows to take")
+        need = L.load().wf_grouped_fp8_workspace_bytes(int(rows is not None), r, e, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _run(dev, "wf_grouped_fp8_gemm", L.ptr(a), L.ptr(a_s), _kind(a_s), L.ptr(w), L.ptr(w_s), _kind(w_s),
-             L.ptr(offsets), L.ptr(rows), m, r, e, n, k, L.ptr(out))
+             L.ptr(offsets), L.ptr(rows), m, r, e, n, k, L.ptr(out), L.ptr(ws), need)
     return out
 
 
