@@ -2,7 +2,9 @@
 
 Usage: ``python -m wanferenz_b200._build`` (or ``__graft_entry__.build()``).
 The library is plain nvcc output with a C ABI (``include/wfb200.h``); it
-statically links the CUDA runtime and is loaded with ctypes.
+statically links the CUDA runtime and is loaded with ctypes.  Beside it goes
+``lib/_wfb200_torch.so``, the compiled Python entry of the operators of
+``csrc/wf_torch.cpp`` (host code, linked to the library and to torch).
 """
 
 from __future__ import annotations
@@ -17,6 +19,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libwfb200.so")
+EXT = os.path.join(LIBDIR, "_wfb200_torch.so")
+EXT_SRC = os.path.join(CSRC, "wf_torch.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -42,27 +46,55 @@ def deps():
         os.path.join(ROOT, "include", "wfb200.h")]
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+def ext_deps():
+    return [EXT_SRC, os.path.join(ROOT, "include", "wfb200.h")]
+
+
+def up_to_date(target: str = LIB, of=None) -> bool:
+    if not os.path.exists(target):
         return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(p) <= t for p in deps())
+    t = os.path.getmtime(target)
+    return all(os.path.getmtime(p) <= t for p in (of or deps()))
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB
-    os.makedirs(LIBDIR, exist_ok=True)
-    tmp = LIB + f".tmp{os.getpid()}"
-    cmd = [nvcc(), *NVCC_FLAGS, "--threads", "0", "-o", tmp, *sources()]
+def _run(cmd, target, verbose):
+    tmp = target + f".tmp{os.getpid()}"
+    cmd = [tmp if c is None else c for c in cmd]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, LIB)
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, target)
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    os.makedirs(LIBDIR, exist_ok=True)
+    if force or not up_to_date():
+        _run([nvcc(), *NVCC_FLAGS, "--threads", "0", "-o", None, *sources()], LIB, verbose)
     return LIB
+
+
+def build_ext(force: bool = False, verbose: bool = False) -> str:
+    """The Python entry module; links ``build()``'s library, which must exist."""
+    if not force and up_to_date(EXT, ext_deps()):
+        return EXT
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unknown-pragmas",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    for d in cpp_extension.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"]]:
+        flags += ["-isystem", d]
+    libs = ["-L" + d for d in cpp_extension.library_paths(device_type="cuda")]
+    libs += ["-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+             "-L" + LIBDIR, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    _run([os.environ.get("CXX", "g++"), *flags, EXT_SRC, "-o", None, *libs], EXT, verbose)
+    return EXT
 
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
+    print(build_ext(force="--force" in sys.argv, verbose=True))

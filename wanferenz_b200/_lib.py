@@ -140,6 +140,31 @@ def load(build_if_missing: bool = True):
     return lib
 
 
+_EXT = None
+
+
+def load_ext(build_if_missing: bool = True):
+    """Loads (building first if needed) the compiled Python entry of the layer operators; raises if it cannot."""
+    global _EXT
+    if _EXT is None:
+        load(build_if_missing)
+        if not os.path.exists(_build.EXT):
+            if not build_if_missing:
+                raise ImportError(f"wanferenz_b200: entry module missing at {_build.EXT}; run "
+                                  f"`python -m wanferenz_b200._build`")
+            _build.build_ext()
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries are the module's)
+
+        spec = importlib.util.spec_from_file_location("_wfb200_torch", _build.EXT)
+        ext = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ext)
+        ext.set_check(check)
+        _EXT = ext
+    return _EXT
+
+
 def check(code: int, fn: str):
     if code != WF_OK:
         msg = _LIB.wf_last_error().decode() if _LIB is not None else ""

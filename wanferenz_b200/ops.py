@@ -171,33 +171,14 @@ class NormQuant(NamedTuple):
     h: Optional[torch.Tensor]   # [.., D] bf16 residual stream (residual given)
 
 
-def _check(name, t, dtypes, device=None, shape=None):
-    """Argument checks shared by the operators below: a CUDA tensor of one of ``dtypes`` (on
-    ``device``, of ``shape``); returns it contiguous."""
-    if not t.is_cuda:
-        raise ValueError("wanferenz_b200 operators run on CUDA tensors only")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t.contiguous()
+_EXT = None
 
 
-def _run(device, name, *args):
-    """Calls entry point ``name`` with ``args`` and the current stream of ``device``, with that device current."""
-    fn = getattr(L.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    if rc:
-        L.check(rc, name)
-
-
-_F32, _BF16, _E4M3, _E8M0 = (torch.float32,), (torch.bfloat16,), (torch.float8_e4m3fn,), (torch.float8_e8m0fnu,)
+def _ext():
+    global _EXT
+    if _EXT is None:
+        _EXT = L.load_ext()
+    return _EXT
 
 
 def rms_norm_quant(x, weight, eps=1e-6, *, residual=None, norm_out=True, scale_fmt=None, scale_dtype=torch.float32):
@@ -214,30 +195,7 @@ def rms_norm_quant(x, weight, eps=1e-6, *, residual=None, norm_out=True, scale_f
     ``MoELayer``) unless ``norm_out=False``, ``h`` when ``residual`` is given.  ``q`` is taken from
     the 32-bit ``n``, so it can differ from ``act_quant(y)`` by that one bf16 rounding.
     """
-    x = _check("x", x, _BF16)
-    dev = x.device
-    if x.dim() < 1:
-        raise ValueError("x must have at least one dimension")
-    d = x.size(-1)
-    if d == 0 or d % 128 or d > 16384:
-        raise ValueError(f"last dim {d} must be a multiple of 128, at most 16384")
-    weight = _check("weight", weight, _F32 + _BF16, dev, (d,))
-    if scale_dtype not in _F32 + _E8M0:
-        raise TypeError(f"unsupported scale dtype {scale_dtype}")
-    if scale_fmt is None and scale_dtype == torch.float8_e8m0fnu:
-        raise ValueError("e8m0 scales need scale_fmt (power-of-two rounding)")
-    h = None
-    if residual is not None:
-        residual = _check("residual", residual, _BF16, dev, x.shape)
-        h = torch.empty_like(x)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    s = torch.empty(*x.shape[:-1], d // 128, dtype=scale_dtype, device=dev)
-    y = torch.empty_like(x) if norm_out else None
-    if x.numel():
-        _run(dev, "wf_rms_norm_quant", L.ptr(x), L.ptr(residual), L.ptr(weight), int(weight.dtype == torch.bfloat16),
-             x.numel() // d, d, float(eps), int(scale_fmt is not None), L.ptr(q), L.ptr(s), _kind(s), L.ptr(y),
-             L.ptr(h))
-    return NormQuant(q, s, y, h)
+    return NormQuant._make(_ext().rms_norm_quant(x, weight, eps, residual, norm_out, scale_fmt is not None, scale_dtype))
 
 
 def route_topk(logits, topk, *, bias=None, score_func="sigmoid", n_groups=1, topk_groups=None, group_score=None,
@@ -257,36 +215,15 @@ def route_topk(logits, topk, *, bias=None, score_func="sigmoid", n_groups=1, top
     weight 0, which ``expert_dispatch`` leaves out.  NaN counts as the largest value and shows
     in the weights.  E up to 512, topk up to 16, n_groups up to 32.
     """
-    logits = _check("logits", logits, _F32 + _BF16)
-    dev = logits.device
-    if logits.dim() != 2:
-        raise ValueError("logits must be [T, E]")
-    t, e = logits.shape
     if score_func not in L.WF_SCORE:
         raise ValueError(f"score_func {score_func!r} is not one of {sorted(L.WF_SCORE)}")
-    if bias is not None:
-        bias = _check("bias", bias, _F32, dev, (e,))
     if group_score is None:
-        group_score = "top2" if bias is not None else "max"
-    if group_score not in ("top2", "max"):
+        group_score = "max" if bias is None else "top2"
+    elif group_score not in ("top2", "max"):
         raise ValueError(f"group_score {group_score!r} is not 'top2' or 'max'")
-    if topk_groups is None:
-        topk_groups = n_groups
-    if renormalize is None:
-        renormalize = score_func != "softmax"
-    if not 1 <= e <= 512:
-        raise ValueError(f"{e} experts: 1 to 512 are supported")
-    if not 1 <= n_groups <= 32 or e % n_groups or not 1 <= topk_groups <= n_groups:
-        raise ValueError(f"n_groups {n_groups} (1 to 32) must divide the {e} experts, topk_groups {topk_groups} lie in it")
-    if not 1 <= topk <= min(16, topk_groups * (e // n_groups)):
-        raise ValueError(f"topk {topk} must be in 1..min(16, experts of topk_groups groups)")
-    w = torch.empty(t, topk, dtype=torch.float32, device=dev)
-    i = torch.empty(t, topk, dtype=torch.int64, device=dev)
-    if t:
-        _run(dev, "wf_route_topk", L.ptr(logits), int(logits.dtype == torch.bfloat16), L.ptr(bias), t, e, topk,
-             L.WF_SCORE[score_func], n_groups, topk_groups, int(group_score == "top2"), int(bool(renormalize)),
-             float(route_scale), L.ptr(w), L.ptr(i))
-    return w, i
+    return _ext().route_topk(logits, topk, bias, L.WF_SCORE[score_func], n_groups,
+                             n_groups if topk_groups is None else topk_groups, group_score == "top2",
+                             score_func != "softmax" if renormalize is None else renormalize, route_scale)
 
 
 def expert_dispatch(indices, n_experts, *, expert_offset=0):
@@ -299,26 +236,7 @@ def expert_dispatch(indices, n_experts, *, expert_offset=0):
     (expert, token, slot).  No host synchronization: ``offsets`` and ``tokens`` are what
     ``grouped_fp8_gemm`` takes, ``slots`` what ``expert_combine`` takes.
     """
-    indices = _check("indices", indices, (torch.int64, torch.int32))
-    dev = indices.device
-    if indices.dim() != 2:
-        raise ValueError("indices must be [T, k]")
-    t, k = indices.shape
-    if not 1 <= k <= 16 or not 1 <= n_experts <= 512 or t * k > 1 << 30:
-        raise ValueError(f"indices [{t}, {k}] over {n_experts} experts: k in 1..16, 1 to 512 experts, at most 2^30 pairs")
-    if not 0 <= expert_offset <= 0x7fffffff - 512:
-        raise ValueError(f"expert_offset {expert_offset} out of range")
-    if not t:
-        z = torch.zeros(n_experts + 1, dtype=torch.int32, device=dev)
-        return z, torch.empty(0, dtype=torch.int32, device=dev), torch.empty(0, k, dtype=torch.int32, device=dev)
-    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
-    tokens = torch.empty(t * k, dtype=torch.int32, device=dev)
-    slots = torch.empty(t, k, dtype=torch.int32, device=dev)
-    need = L.load().wf_expert_dispatch_workspace_bytes(t, k, n_experts)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _run(dev, "wf_expert_dispatch", L.ptr(indices), int(indices.dtype == torch.int64), t, k, n_experts, expert_offset,
-         L.ptr(offsets), L.ptr(tokens), L.ptr(slots), L.ptr(ws), need)
-    return offsets, tokens, slots
+    return _ext().expert_dispatch(indices, n_experts, expert_offset)
 
 
 def grouped_fp8_gemm(a, a_s, w, w_s, offsets, *, rows=None, out=None):
@@ -335,38 +253,7 @@ def grouped_fp8_gemm(a, a_s, w, w_s, offsets, *, rows=None, out=None):
     Returns bf16 ``[R, N]`` (``out`` when given); rows behind ``offsets[E]`` are not written.  An
     entry of ``rows`` outside ``[0, M)`` gives a row of zeros.  N a multiple of 8, K of 128.
     """
-    a = _check("a", a, _E4M3)
-    dev = a.device
-    if a.dim() != 2 or w.dim() != 3 or offsets.dim() != 1:
-        raise ValueError("a must be [M, K], w [E, N, K] and offsets [E + 1]")
-    m, k = a.shape
-    e, n, _ = w.shape
-    if k == 0 or k % 128 or k > 1 << 20 or n == 0 or n % 8 or n > 1 << 20 or not 1 <= e <= 512 or e * n > 1 << 30:
-        raise ValueError(f"E {e}, N {n}, K {k}: E in 1..512, N a multiple of 8, K a multiple of 128 (at most 2^20 each)")
-    w = _check("w", w, _E4M3, dev, (e, n, k))
-    a_s = _check("a_s", a_s, _F32 + _E8M0, dev, (m, k // 128))
-    w_s = _check("w_s", w_s, _F32 + _E8M0, dev, (e, (n + 127) // 128, k // 128))
-    offsets = _check("offsets", offsets, (torch.int32,), dev, (e + 1,))
-    r = m
-    if rows is not None:
-        rows = _check("rows", rows, (torch.int32,), dev)
-        if rows.dim() != 1:
-            raise ValueError("rows must be [R]")
-        r = rows.size(0)
-    if m > 1 << 30 or r > 1 << 30:
-        raise ValueError(f"{m} rows of a, {r} rows: at most 2^30 are supported")
-    if out is None:
-        out = torch.empty(r, n, dtype=torch.bfloat16, device=dev)
-    elif _check("out", out, _BF16, dev, (r, n)) is not out:
-        raise ValueError("out must be contiguous")
-    if r:
-        if not m:
-            raise ValueError("a has no rows to take")
-        need = L.load().wf_grouped_fp8_workspace_bytes(int(rows is not None), r, e, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _run(dev, "wf_grouped_fp8_gemm", L.ptr(a), L.ptr(a_s), _kind(a_s), L.ptr(w), L.ptr(w_s), _kind(w_s),
-             L.ptr(offsets), L.ptr(rows), m, r, e, n, k, L.ptr(out), L.ptr(ws), need)
-    return out
+    return _ext().grouped_fp8_gemm(a, a_s, w, w_s, offsets, rows, out)
 
 
 def grouped_read_error(device=None):
@@ -384,26 +271,7 @@ def expert_combine(rows, slots, *, weights=None, shared=None, out_dtype=torch.bf
     is ascending expert, as MoE.forward's does (architecture.py:785-794).  ``out_dtype``
     ``torch.float32`` gives a rank's partial sum (``MoELayer.sum_ranks`` adds those).
     """
-    rows = _check("rows", rows, _BF16)
-    dev = rows.device
-    slots = _check("slots", slots, (torch.int32,), dev)
-    if rows.dim() != 2 or slots.dim() != 2:
-        raise ValueError("rows must be [R, D] and slots [T, k]")
-    r, d = rows.shape
-    t, k = slots.shape
-    if d == 0 or d % 8 or d > 1 << 20 or not 1 <= k <= 16 or r > 0x7fffffff:
-        raise ValueError(f"rows [{r}, {d}], slots [{t}, {k}]: D must be a multiple of 8 up to 2^20, k in 1..16")
-    if weights is not None:
-        weights = _check("weights", weights, _F32, dev, (t, k))
-    if shared is not None:
-        shared = _check("shared", shared, _BF16, dev, (t, d))
-    if out_dtype not in _BF16 + _F32:
-        raise TypeError(f"out_dtype {out_dtype} is not bfloat16 or float32")
-    y = torch.empty(t, d, dtype=out_dtype, device=dev)
-    if t:
-        _run(dev, "wf_expert_combine", L.ptr(rows), r, L.ptr(slots), L.ptr(weights), L.ptr(shared), t, k, d, L.ptr(y),
-             int(out_dtype == torch.float32))
-    return y
+    return _ext().expert_combine(rows, slots, weights, shared, out_dtype)
 
 
 OPERATORS = {
