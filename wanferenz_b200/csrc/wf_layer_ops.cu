@@ -172,7 +172,10 @@ __global__ void __launch_bounds__(256) k_rms_norm_quant(const __grid_constant__ 
 // -infinity masks its expert: it is never chosen, and slots that find no expert
 // get index -1 and weight 0.  NaN counts as the largest value, as in torch.topk,
 // so it shows in the weights.
-// One warp per token; a lane holds experts lane, lane + 32, ...
+// One warp per token; a lane holds experts lane, lane + 32, ...  Scores of sigmoid and
+// sqrt(softplus) are screened in 32 bits first (route32); rows whose choice 32 bits
+// cannot settle, and softmax, take the 64-bit path (route64).  The chosen experts'
+// weights are in 64 bits on both.
 // ---------------------------------------------------------------------------
 constexpr int ROUTE_MAX_E = 512, ROUTE_MAX_K = 16, ROUTE_MAX_G = 32;
 constexpr int ROUTE_WARPS = 4;
@@ -204,25 +207,24 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
     return (unsigned long long)hi << 32 | lo;
 }
 
-template <int N>  // experts per lane
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route_topk(const __grid_constant__ RouteArgs p) {
-    __shared__ double picked[ROUTE_WARPS][ROUTE_MAX_K];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long t = (long long)blockIdx.x * ROUTE_WARPS + warp;
-    if (t >= p.T) return;
+// One score in 64 bits (sigmoid, sqrt(softplus); softmax needs the row).
+__device__ __forceinline__ double score64(double z, int score) {
+    if (score == WF_SCORE_SIGMOID) return 1.0 / (1.0 + exp(-z));
+    return sqrt((z > 0 ? z : 0.0) + log1p(exp(-fabs(z))));
+}
+
+// The whole choice in 64 bits; lane j < k returns the expert of slot j in my_idx (-1: none) and its score.
+template <int N>
+__device__ __noinline__ double route64(const RouteArgs &p, const float (&zf)[N], int &my_idx) {
+    const int lane = threadIdx.x & 31;
     double s[N];
     unsigned long long key[N];
     double top = -CUDART_INF;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int e = lane + 32 * i;
-        float z = -CUDART_INF_F;
-        if (e < p.E)
-            z = p.bf16 ? __bfloat162float(((const __nv_bfloat16 *)p.logits)[t * p.E + e])
-                       : ((const float *)p.logits)[t * p.E + e];
-        s[i] = z;
-        nan |= z != z;
+        s[i] = zf[i];
+        nan |= zf[i] != zf[i];
         top = fmax(top, s[i]);
     }
     if (p.score == WF_SCORE_SOFTMAX) {
@@ -244,10 +246,8 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route_topk(const __grid_co
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const double z = s[i];
-            key[i] = z != -CUDART_INF;
-            if (p.score == WF_SCORE_SIGMOID) s[i] = 1.0 / (1.0 + exp(-z));
-            else s[i] = sqrt((z > 0 ? z : 0.0) + log1p(exp(-fabs(z))));
+            key[i] = s[i] != -CUDART_INF;
+            s[i] = score64(s[i], p.score);
         }
     }
 #pragma unroll
@@ -281,8 +281,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route_topk(const __grid_co
             }
             if (lane == g) mine = gv;
         }
-        // keep the best groups: one flag bit each
-        uint32_t kept = 0;
+        uint32_t kept = 0;  // one bit per group
         for (int j = 0; j < p.keep; ++j) {
             const unsigned long long m = warp_max(mine);
             if (!m) break;
@@ -296,40 +295,173 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route_topk(const __grid_co
             if (e < p.E && !(kept >> (e / per) & 1)) key[i] = 0;
         }
     }
-    int my_idx = -1;
+    my_idx = -1;
+    double mine = 0.0;
     for (int j = 0; j < p.k; ++j) {
         unsigned long long a = 0;
-        int at = 0;
+        double sa = 0.0;
+        int e = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (key[i] > a) { a = key[i]; at = i; }
+            if (key[i] > a) { a = key[i]; sa = s[i]; e = lane + 32 * i; }
         const unsigned long long m = warp_max(a);
-        if (!m) {
-            if (lane >= j && lane < p.k) picked[warp][lane] = 0.0;
-            break;
-        }
-        const int e = lane + 32 * at;
+        if (!m) break;
         const uint32_t best = __reduce_min_sync(0xffffffffu, a == m ? (uint32_t)e : 0xffffffffu);
-        if (a == m && (uint32_t)e == best) {
+        const double sb = __shfl_sync(0xffffffffu, sa, best & 31);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i == at) {
-                    key[i] = 0;
-                    picked[warp][j] = s[i];
-                }
+        for (int i = 0; i < N; ++i)
+            if ((uint32_t)(lane + 32 * i) == best) key[i] = 0;
+        if (lane == j) {
+            my_idx = (int)best;
+            mine = sb;
         }
-        if (lane == j) my_idx = (int)best;
     }
-    __syncwarp();
-    if (lane < p.k) {
-        double w = picked[warp][lane];
-        if (p.renorm) {
-            double sum = 0.0;
-            for (int j = 0; j < p.k; ++j) sum += picked[warp][j];
-            w = sum == 0.0 ? 0.0 : w / sum;
+    return mine;
+}
+
+// 32-bit keys: order kept under unsigned comparison, 0 below every value
+__device__ __forceinline__ uint32_t key32(float f) {
+    const uint32_t b = __float_as_uint(f);
+    return b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float value32(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// The choice screened in 32 bits.  A 32-bit score is off by less than 2^-21 of itself (expf and
+// log1pf to 2 ulp, an addition, a division or a square root) and sel by half an ulp more, so two
+// values further apart than `gap` are in the right order; where any decision of the row (a slot
+// against the next, the last group kept against the first dropped) is closer than that, or the
+// row has NaN, +infinity or too few experts, the row is left to route64.  Returns whether all
+// decisions stand; lane j < k has the expert of slot j.
+template <int N>
+__device__ __forceinline__ bool route32(const RouteArgs &p, const float (&z)[N], uint32_t *sm, int &my_idx) {
+    const int lane = threadIdx.x & 31;
+    uint32_t key[N];
+    float smax = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = lane + 32 * i;
+        odd |= !(z[i] < CUDART_INF_F);
+        float sc;
+        if (p.score == WF_SCORE_SIGMOID) sc = __frcp_rn(1.0f + expf(-z[i]));
+        else sc = __fsqrt_rn(fmaxf(z[i], 0.f) + log1pf(expf(-fabsf(z[i]))));
+        smax = fmaxf(smax, sc);
+        const float sel = p.bias && e < p.E ? sc + __ldg(p.bias + e) : sc;
+        odd |= !(sel < CUDART_INF_F);
+        key[i] = z[i] == -CUDART_INF_F || sel == -CUDART_INF_F ? 0u : key32(sel + 0.0f);
+    }
+    if (__any_sync(0xffffffffu, odd)) return false;
+    smax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)));  // scores are not negative
+    if (smax < 0x1p-40f) return false;  // subnormal steps of expf: the bound above does not hold
+    const float gap0 = smax * 0x1p-18f;
+    if (p.G > 1) {
+        // 2^w lanes per group: each takes every 2^w-th expert of it, then their best two are merged
+        const int per = p.E / p.G, w = 31 - __clz(32 / p.G), sub = lane & ((1 << w) - 1), grp = lane >> w;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (lane + 32 * i < p.E) sm[lane + 32 * i] = key[i];
+        __syncwarp();
+        uint32_t a = 0, b = 0;
+        if (grp < p.G) {
+            for (int j = sub; j < per; j += 1 << w) {
+                const uint32_t v = sm[grp * per + j];
+                b = max(b, min(a, v));
+                a = max(a, v);
+            }
         }
-        p.w[t * p.k + lane] = (float)(my_idx < 0 ? 0.0 : w * p.scale);
-        p.idx[t * p.k + lane] = my_idx;
+        for (int o = 1; o < 1 << w; o <<= 1) {
+            const uint32_t a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+            b = max(min(a, a2), max(b, b2));
+            a = max(a, a2);
+        }
+        // a sum's error goes with its terms, which may cancel
+        const float mag = __uint_as_float(__reduce_max_sync(
+            0xffffffffu, max(a ? __float_as_uint(fabsf(value32(a))) : 0u, b ? __float_as_uint(fabsf(value32(b))) : 0u)));
+        uint32_t mine = a;
+        if (p.top2 && b) {
+            const float v = value32(a) + value32(b);
+            mine = v > -CUDART_INF_F ? key32(v + 0.0f) : 0u;
+        }
+        if (sub) mine = 0;
+        uint32_t kept = 0, m = 0;
+        for (int j = 0; j < p.keep; ++j) {
+            m = __reduce_max_sync(0xffffffffu, mine);
+            if (!m) return false;
+            const int who = __ffs(__ballot_sync(0xffffffffu, mine == m)) - 1;
+            kept |= 1u << (who >> w);
+            if (lane == who) mine = 0;
+        }
+        const uint32_t next = __reduce_max_sync(0xffffffffu, mine);
+        if (next) {
+            if (!(value32(m) - value32(next) > 2 * gap0 + mag * 0x1p-18f)) return false;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = lane + 32 * i;
+            if (e < p.E && !(kept >> (e / per) & 1)) key[i] = 0;
+        }
+    }
+    my_idx = -1;
+    float last = 0.f;
+    for (int j = 0; j <= p.k; ++j) {
+        uint32_t a = 0;
+        int e = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (key[i] > a) { a = key[i]; e = lane + 32 * i; }
+        const uint32_t m = __reduce_max_sync(0xffffffffu, a);
+        if (!m) return j == p.k;
+        const float v = value32(m);
+        if (j > 0 && !(last - v > gap0 + fmaxf(fabsf(last), fabsf(v)) * 0x1p-18f)) return false;
+        if (j == p.k) break;
+        last = v;
+        const int who = __ffs(__ballot_sync(0xffffffffu, a == m)) - 1;
+        const int best = __shfl_sync(0xffffffffu, e, who);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (lane + 32 * i == best) key[i] = 0;
+        if (lane == j) my_idx = best;
+    }
+    return true;
+}
+
+template <int N>  // experts per lane
+__global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route_topk(const __grid_constant__ RouteArgs p) {
+    __shared__ uint32_t sm[ROUTE_WARPS][32 * N];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long t = (long long)blockIdx.x * ROUTE_WARPS + warp;
+    if (t >= p.T) return;
+    float z[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = lane + 32 * i;
+        z[i] = -CUDART_INF_F;
+        if (e < p.E)
+            z[i] = p.bf16 ? __bfloat162float(((const __nv_bfloat16 *)p.logits)[t * p.E + e])
+                          : __ldg((const float *)p.logits + t * p.E + e);
+    }
+    int idx = -1;
+    double s;
+    // softmax weights need the row's sum in 64 bits anyway
+    if (p.score != WF_SCORE_SOFTMAX && route32<N>(p, z, sm[warp], idx)) {
+        const long long at = t * p.E + max(idx, 0);
+        s = idx < 0 ? 0.0
+                    : score64(p.bf16 ? (double)__bfloat162float(((const __nv_bfloat16 *)p.logits)[at])
+                                     : (double)__ldg((const float *)p.logits + at),
+                              p.score);
+    } else {
+        s = route64<N>(p, z, idx);
+    }
+    if (p.renorm) {
+        double sum = 0.0;  // the same order in every lane
+        for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, s, j);
+        s = sum == 0.0 ? 0.0 : s / sum;
+    }
+    if (lane < p.k) {
+        p.w[t * p.k + lane] = (float)(idx < 0 ? 0.0 : s * p.scale);
+        p.idx[t * p.k + lane] = idx;
     }
 }
 
@@ -343,85 +475,116 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route_topk(const __grid_co
 // warp counts its run per expert (lanes that hold the same expert find one
 // another with match_any), the counts are summed over warps and chunks, and a
 // second walk over the run hands out the places.  One launch where one chunk
-// holds all pairs, else a counting launch before it.
+// holds all pairs; else a counting launch before it, under which this one starts
+// (programmatic launch) and reads and counts its own run.
+// Latency-bound at every size (16384 x 8 pairs are 2 MB): a warp's pairs sit in
+// registers, 4 loads in flight, and the two walks read no memory.
 // ---------------------------------------------------------------------------
-constexpr int DISP_MAX_E = 512, DISP_WARPS = 8, DISP_MAX_CHUNKS = 256, DISP_CHUNK = 2048;
+constexpr int DISP_MAX_E = 512, DISP_WARPS = 16, DISP_LANE = 4, DISP_STEP = 32 * DISP_LANE;  // pairs of a warp's step
+constexpr int DISP_CHUNK = DISP_WARPS * DISP_STEP, DISP_MAX_CHUNKS = 512;
 
 struct DispArgs {
     const void *indices;
     int idx64;
     int pairs, k, E, base;
-    int chunk, nchunks;
-    int *hist;  // [nchunks, E] when nchunks > 1
+    int run, nchunks;  // pairs per warp (a multiple of 32), chunks of DISP_WARPS runs
+    int *hist;         // [nchunks, E] when nchunks > 1
     int *offsets, *tokens, *slots;
 };
 
-__device__ __forceinline__ int disp_expert(const DispArgs &p, int i) {
-    const long long e = (p.idx64 ? ((const long long *)p.indices)[i] : (long long)((const int *)p.indices)[i]) - p.base;
-    return e >= 0 && e < p.E ? (int)e : -1;
-}
-
-// per-warp counts of a chunk into cnt[warp][E]
-__device__ __forceinline__ void disp_count(const DispArgs &p, int lo, int hi, int *cnt) {
+// The local experts of DISP_LANE x 32 consecutive pairs from i0 on (-1: none), pair i0 + 32 j + lane in e[j].
+__device__ __forceinline__ void disp_load(const DispArgs &p, int i0, int hi, int (&e)[DISP_LANE]) {
     const int lane = threadIdx.x & 31;
-    for (int e = lane; e < p.E; e += 32) cnt[e] = 0;
-    __syncwarp();
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < hi ? disp_expert(p, i) : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && lane == __ffs(same) - 1) cnt[e] += __popc(same);
-        __syncwarp();
+    long long v[DISP_LANE];
+#pragma unroll
+    for (int j = 0; j < DISP_LANE; ++j) {
+        const int i = i0 + 32 * j + lane;
+        v[j] = -1;
+        if (i < hi) v[j] = p.idx64 ? __ldg((const long long *)p.indices + i) : (long long)__ldg((const int *)p.indices + i);
+    }
+#pragma unroll
+    for (int j = 0; j < DISP_LANE; ++j) {
+        const int i = i0 + 32 * j + lane;
+        e[j] = i < hi && v[j] >= p.base && v[j] < (long long)p.base + p.E ? (int)(v[j] - p.base) : -1;
     }
 }
 
 __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_count(const __grid_constant__ DispArgs p) {
-    __shared__ int cnt[DISP_WARPS][DISP_MAX_E];
+    __shared__ int cnt[DISP_MAX_E];
+    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5;
-    const int run = p.chunk / DISP_WARPS;
-    const int lo = min(p.pairs, blockIdx.x * p.chunk + warp * run), hi = min(p.pairs, lo + run);
-    disp_count(p, lo, hi, cnt[warp]);
+    const int lo = min(p.pairs, (blockIdx.x * DISP_WARPS + warp) * p.run), hi = min(p.pairs, lo + p.run);
+    int e[DISP_LANE];
+    disp_load(p, lo, hi, e);
+    for (int x = threadIdx.x; x < p.E; x += blockDim.x) cnt[x] = 0;
     __syncthreads();
-    for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-        int n = 0;
+    for (int i0 = lo; i0 < hi;) {
 #pragma unroll
-        for (int w = 0; w < DISP_WARPS; ++w) n += cnt[w][e];
-        p.hist[(size_t)blockIdx.x * p.E + e] = n;
+        for (int j = 0; j < DISP_LANE; ++j)
+            if (e[j] >= 0) atomicAdd(&cnt[e[j]], 1);
+        i0 += DISP_STEP;
+        if (i0 < hi) disp_load(p, i0, hi, e);
     }
+    __syncthreads();
+    for (int x = threadIdx.x; x < p.E; x += blockDim.x) p.hist[(size_t)blockIdx.x * p.E + x] = cnt[x];
 }
 
 __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid_constant__ DispArgs p) {
     __shared__ int cnt[DISP_WARPS][DISP_MAX_E];
-    __shared__ int total[DISP_MAX_E + 1], scan[DISP_WARPS];
+    __shared__ int total[DISP_MAX_E + 1], before[DISP_MAX_E], scan[DISP_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int run = p.chunk / DISP_WARPS;
-    const int lo = min(p.pairs, blockIdx.x * p.chunk + warp * run), hi = min(p.pairs, lo + run);
-    disp_count(p, lo, hi, cnt[warp]);
-    __syncthreads();
-    // each warp's start within the expert, relative to the expert's first row
-    for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-        int before = 0, all = 0;
-        if (p.nchunks > 1) {
-            for (int c = 0; c < p.nchunks; ++c) {
-                const int n = p.hist[(size_t)c * p.E + e];
-                if (c < (int)blockIdx.x) before += n;
-                all += n;
-            }
-        }
+    const int lo = min(p.pairs, (blockIdx.x * DISP_WARPS + warp) * p.run), hi = min(p.pairs, lo + p.run);
+    const bool whole = hi - lo <= DISP_STEP;  // the run stays in registers
+    int e[DISP_LANE], ahead[DISP_LANE];
+    disp_load(p, lo, hi, e);
+    for (int x = lane; x < p.E; x += 32) cnt[warp][x] = 0;
+    for (int x = threadIdx.x; x < p.E; x += blockDim.x) total[x] = before[x] = 0;
+    __syncwarp();
+    for (int i0 = lo; i0 < hi;) {
 #pragma unroll
-        for (int w = 0; w < DISP_WARPS; ++w) {
-            const int n = cnt[w][e];
-            cnt[w][e] = before;
-            before += n;
+        for (int j = 0; j < DISP_LANE; ++j) {
+            // pairs of the same expert earlier in the run: this warp's so far, then lower lanes
+            const uint32_t same = __match_any_sync(0xffffffffu, e[j]);
+            const int at = e[j] >= 0 ? cnt[warp][e[j]] : 0;
+            ahead[j] = at + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (e[j] >= 0 && lane == __ffs(same) - 1) cnt[warp][e[j]] = at + __popc(same);
+            __syncwarp();
         }
-        total[e] = p.nchunks > 1 ? all : before;
+        i0 += DISP_STEP;
+        if (i0 < hi) disp_load(p, i0, hi, e);
+    }
+    if (p.nchunks > 1) {
+        __syncthreads();
+        pdl_wait();
+        for (int x = lane; x < p.E; x += 32) {
+            int pre = 0, all = 0;
+#pragma unroll 4
+            for (int c = warp; c < p.nchunks; c += DISP_WARPS) {
+                const int n = __ldcg(p.hist + (size_t)c * p.E + x);
+                all += n;
+                if (c < (int)blockIdx.x) pre += n;
+            }
+            if (all) atomicAdd(&total[x], all);
+            if (pre) atomicAdd(&before[x], pre);
+        }
     }
     __syncthreads();
-    // exclusive scan of the experts' totals: two neighbouring experts per thread
+    // expert x (one thread each): where each warp's pairs of it start, and where the expert starts
     {
-        const int e0 = 2 * threadIdx.x;
-        const int a = e0 < p.E ? total[e0] : 0, b = e0 + 1 < p.E ? total[e0 + 1] : 0;
-        int incl = a + b;
+        const int x = threadIdx.x;
+        int at = 0, all = 0;
+        if (x < p.E) {
+            at = before[x];
+#pragma unroll
+            for (int w = 0; w < DISP_WARPS; ++w) {
+                const int n = cnt[w][x];
+                cnt[w][x] = at;
+                at += n;
+            }
+            all = p.nchunks > 1 ? total[x] : at;
+        }
+        int incl = all;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -429,31 +592,34 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid
         }
         if (lane == 31) scan[warp] = incl;
         __syncthreads();
-        int at = incl - a - b;
-        for (int w = 0; w < warp; ++w) at += scan[w];
-        if (e0 <= p.E) total[e0] = at;
-        if (e0 + 1 <= p.E) total[e0 + 1] = at + a;
-        if (threadIdx.x == blockDim.x - 1 && p.E == DISP_MAX_E) total[p.E] = at + a + b;
+        int start = incl - all;
+        for (int w = 0; w < warp; ++w) start += scan[w];
+        if (x <= p.E) total[x] = start;
+        if (x == DISP_MAX_E - 1 && p.E == DISP_MAX_E) total[DISP_MAX_E] = start + all;
     }
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = total[e];
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < hi ? disp_expert(p, i) : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        int at = 0;
-        if (e >= 0) at = cnt[warp][e];
-        __syncwarp();
-        if (e >= 0 && lane == __ffs(same) - 1) cnt[warp][e] = at + __popc(same);
-        __syncwarp();
-        if (i < hi) {
+        for (int x = threadIdx.x; x <= p.E; x += blockDim.x) p.offsets[x] = total[x];
+    for (int i0 = lo; i0 < hi; i0 += DISP_STEP) {
+        if (!whole) disp_load(p, i0, hi, e);
+#pragma unroll
+        for (int j = 0; j < DISP_LANE; ++j) {
+            const int i = i0 + 32 * j + lane;
             int r = -1;
-            if (e >= 0) {
-                r = total[e] + at + __popc(same & ((1u << lane) - 1));
-                p.tokens[r] = i / p.k;
+            if (whole) {
+                if (e[j] >= 0) r = total[e[j]] + cnt[warp][e[j]] + ahead[j];
+            } else {
+                const uint32_t same = __match_any_sync(0xffffffffu, e[j]);
+                const int at = e[j] >= 0 ? cnt[warp][e[j]] : 0;
+                __syncwarp();
+                if (e[j] >= 0 && lane == __ffs(same) - 1) cnt[warp][e[j]] = at + __popc(same);
+                __syncwarp();
+                if (e[j] >= 0) r = total[e[j]] + at + __popc(same & ((1u << lane) - 1));
             }
-            p.slots[i] = r;
+            if (i < hi) {
+                if (r >= 0) p.tokens[r] = i / p.k;
+                p.slots[i] = r;
+            }
         }
     }
     // rows that no pair of the range fills
@@ -612,35 +778,42 @@ int wf_route_topk(const void *logits, int32_t logits_bf16, const float *bias, in
     return launched("route_topk launch");
 }
 
-static int disp_chunks(int64_t pairs, int *chunk) {
-    int64_t c = DISP_CHUNK;
-    if (pairs > c * DISP_MAX_CHUNKS) {
-        c = (pairs + DISP_MAX_CHUNKS - 1) / DISP_MAX_CHUNKS;
-        c = (c + 32 * DISP_WARPS - 1) / (32 * DISP_WARPS) * (32 * DISP_WARPS);
+// Chunks of `pairs` pairs, and the pairs of a warp's run: short runs for few pairs, so that the
+// warps of the one CTA share them, longer than a step only past DISP_MAX_CHUNKS full chunks.
+static int disp_chunks(int64_t pairs, int *run) {
+    int64_t r = DISP_STEP;
+    if (pairs <= DISP_CHUNK) {
+        r = (pairs + DISP_WARPS - 1) / DISP_WARPS;
+        r = (r + 31) / 32 * 32;
+    } else if (pairs > (int64_t)DISP_CHUNK * DISP_MAX_CHUNKS) {
+        r = (pairs + (int64_t)DISP_MAX_CHUNKS * DISP_WARPS - 1) / (DISP_MAX_CHUNKS * DISP_WARPS);
+        r = (r + DISP_STEP - 1) / DISP_STEP * DISP_STEP;
     }
-    *chunk = (int)c;
-    return (int)((pairs + c - 1) / c);
+    *run = (int)r;
+    return (int)((pairs + r * DISP_WARPS - 1) / (r * DISP_WARPS));
+}
+
+static bool disp_ok(int64_t T, int32_t topk, int32_t n_experts) {
+    return T > 0 && topk > 0 && topk <= ROUTE_MAX_K && T <= 1 << 30 && T * topk <= 1 << 30 && n_experts > 0 &&
+           n_experts <= DISP_MAX_E;
 }
 
 size_t wf_expert_dispatch_workspace_bytes(int64_t T, int32_t topk, int32_t n_experts) {
-    if (T <= 0 || topk <= 0 || topk > ROUTE_MAX_K || T > (1 << 30) || T * topk > (1 << 30) || n_experts <= 0 ||
-        n_experts > DISP_MAX_E) {
-        fail(WF_E_SHAPE, "need topk in 1..16, T * topk in 1..2^30 and n_experts in 1..512");
-        return 0;
-    }
-    int chunk;
-    const int n = disp_chunks(T * topk, &chunk);
-    return n > 1 ? (size_t)n * n_experts * 4 : 16;
+    if (!disp_ok(T, topk, n_experts)) return 0;
+    int run;
+    const int n = disp_chunks(T * topk, &run);
+    return n > 1 ? (size_t)n * n_experts * 4 : 0;
 }
 
 int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32_t topk, int32_t n_experts,
                        int64_t expert_offset, int32_t *offsets, int32_t *tokens, int32_t *slots, void *workspace,
                        size_t workspace_bytes, void *stream) {
-    if (!indices || !offsets || !tokens || !slots || !workspace) return fail(WF_E_ARG, "null pointer");
-    const size_t need = wf_expert_dispatch_workspace_bytes(T, topk, n_experts);
-    if (!need) return WF_E_SHAPE;
+    if (!indices || !offsets || !tokens || !slots) return fail(WF_E_ARG, "null pointer");
+    if (!disp_ok(T, topk, n_experts))
+        return fail(WF_E_SHAPE, "need topk in 1..16, T * topk in 1..2^30 and n_experts in 1..512");
     if (expert_offset < 0 || expert_offset > 0x7fffffff - DISP_MAX_E) return fail(WF_E_SHAPE, "expert_offset out of range");
-    if (workspace_bytes < need)
+    const size_t need = wf_expert_dispatch_workspace_bytes(T, topk, n_experts);
+    if (need && (!workspace || workspace_bytes < need))
         return fail(WF_E_ARG, "workspace too small (see wf_expert_dispatch_workspace_bytes)");
     if (misaligned(indices, indices_64 ? 8 : 4) || misaligned(offsets, 4) || misaligned(tokens, 4) ||
         misaligned(slots, 4) || misaligned(workspace, 4))
@@ -648,15 +821,26 @@ int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32
     DispArgs p;
     p.indices = indices; p.idx64 = indices_64 != 0; p.pairs = (int)(T * topk); p.k = topk; p.E = n_experts;
     p.base = (int)expert_offset; p.hist = (int *)workspace; p.offsets = offsets; p.tokens = tokens; p.slots = slots;
-    p.nchunks = disp_chunks(p.pairs, &p.chunk);
+    p.nchunks = disp_chunks(p.pairs, &p.run);
     cudaStream_t st = (cudaStream_t)stream;
-    if (p.nchunks > 1) {
-        k_dispatch_count<<<p.nchunks, 32 * DISP_WARPS, 0, st>>>(p);
+    if (p.nchunks == 1) {
+        k_dispatch_place<<<1, 32 * DISP_WARPS, 0, st>>>(p);
         wf::host::counted();
+        return launched("expert_dispatch launch");
     }
-    k_dispatch_place<<<p.nchunks, 32 * DISP_WARPS, 0, st>>>(p);
-    wf::host::counted();
-    return launched("expert_dispatch launch");
+    k_dispatch_count<<<p.nchunks, 32 * DISP_WARPS, 0, st>>>(p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.nchunks);
+    cfg.blockDim = dim3(32 * DISP_WARPS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_dispatch_place, p);
+    wf::host::counted(2);
+    return e == cudaSuccess ? launched("expert_dispatch launch") : cuda_fail(e, "expert_dispatch launch");
 }
 
 int wf_expert_combine(const void *rows, int64_t R, const int32_t *slots, const float *weights, const void *shared,

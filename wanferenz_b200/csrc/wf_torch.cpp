@@ -211,7 +211,8 @@ WF_ENTRY(expert_dispatch, 3) {
     if (!t) return pack({at::zeros({n + 1}, at::TensorOptions(dev).dtype(at::kInt)), tokens, slots});
     const at::Tensor offsets = empty({n + 1}, at::kInt, dev);
     const size_t need = wf_expert_dispatch_workspace_bytes(t, (int32_t)k, (int32_t)n);
-    const at::Tensor ws = empty({(int64_t)need}, at::kByte, dev);
+    at::Tensor ws;
+    if (need) ws = empty({(int64_t)need}, at::kByte, dev);
     run(dev, "wf_expert_dispatch", [&](void *stream) {
         return wf_expert_dispatch(ptr(x), x.scalar_type() == at::kLong, t, (int32_t)k, (int32_t)n, base, (int32_t *)ptr(offsets),
                                   (int32_t *)ptr(tokens), (int32_t *)ptr(slots), ptr(ws), need, stream);
