@@ -481,3 +481,38 @@ def test_refusals():
         with pytest.raises(err):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "sqrtsoftplus"])
+@pytest.mark.parametrize("bits", [6, 12, 20])
+def test_route_topk_close_calls(score, bits):
+    """Logits on coarse grids and pairs one step apart: many slots and groups that 32 bits cannot tell apart."""
+    g = _gen(17, bits)
+    base = torch.randn(96, 64, generator=g, device="cuda")
+    logits = (base * 2 ** bits).round() / 2 ** bits
+    # every second expert of the first half a neighbour of the one before it
+    up = torch.nextafter(logits[:48, ::2], torch.full_like(logits[:48, ::2], math.inf))
+    logits[:48, 1::2] = torch.where(torch.rand(48, 32, generator=g, device="cuda") < 0.5, up, logits[:48, ::2])
+    # groups that mirror one another up to a step
+    logits[48:, 32:] = logits[48:, :32]
+    logits[72:, 33] = torch.nextafter(logits[72:, 33], torch.full_like(logits[72:, 33], math.inf))
+    bias = torch.randn(64, generator=g, device="cuda") * 0.01
+    bias[32:] = bias[:32]
+    for b in (None, bias):
+        for G, keep, top2 in ((1, 1, True), (8, 3, True), (8, 5, False), (4, 2, True), (32, 9, True)):
+            _check_route(logits, 6, b, score, G, keep, top2)
+
+
+def test_route_topk_large_and_cancelling_biases():
+    """Biases that dwarf the scores, and pairs that cancel in a group's sum, leave the choice exact."""
+    g = _gen(18)
+    logits = torch.randn(64, 64, generator=g, device="cuda")
+    bias = torch.zeros(64, device="cuda")
+    bias[::8] = 1000.0
+    bias[1::8] = -1000.0
+    _check_route(logits, 6, bias, "sigmoid", 8, 4)
+    bias = torch.full((64,), -1e9, device="cuda")
+    bias[:20] = 0
+    _check_route(logits, 8, bias, "sigmoid", 8, 4)
+    _check_route(logits - 100, 8, None, "sqrtsoftplus")
+    _check_route(logits - 95, 8, None, "sigmoid")

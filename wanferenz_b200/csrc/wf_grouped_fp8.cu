@@ -32,29 +32,36 @@ using namespace tc;
 __device__ int g_err;  // error flags of the grouped products since the last wf_grouped_read_error
 
 constexpr int MAX_E = 512;
-constexpr int NT = 256;                                  // tokens per tile, at most
-constexpr int STAGES = 6;
-constexpr int ABYTES = 128 * 128, BBYTES = NT / 2 * 128, STAGE = ABYTES + BBYTES;
-constexpr int SGRP = 8;                                  // K steps per group of scales
-constexpr int GATHER_ROWS = 64;                          // rows per expert up to which row lists are gathered in place
+constexpr int SGRP = 8;                 // K steps per group of scales
+constexpr int FEW = 64;                 // rows per expert up to which tiles are narrow and row lists gathered in place
 constexpr int W_PROD = 0, W_MMA = 1, WORKERS = 8;
-constexpr int NBAR = 2 * STAGES + 9;
-constexpr int OFF_S = STAGES * STAGE;                    // scales: [2][SGRP][NT] f32 or [2][NT] x 8 bytes
-constexpr int OFF_LO = OFF_S + 2 * SGRP * NT * 4;        // [MAX_E] first row
-constexpr int OFF_CNT = OFF_LO + MAX_E * 4;              // [MAX_E] rows
-constexpr int OFF_T = OFF_CNT + MAX_E * 4;               // [MAX_E + 1] first token tile
-constexpr int OFF_BAR = OFF_T + (MAX_E + 4) * 4;
-constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
-static_assert(SMEM <= 232448 && OFF_BAR % 8 == 0, "shared memory");
-// TMEM columns: the tile's sums and two groups of scale factors (e8m0), or two step products (f32)
-constexpr uint32_t COL_SFA = 256, COL_SFB = 320;
+constexpr int SMEM_MAX = 232448;
 
-// e8m0: 4 scale warps (one per TMEM lane quadrant); f32: 2, and the workers' accumulators need
-// the registers of a smaller block.
-template <bool E8>
-struct Roles {
+// One kernel per way of applying scales and per tile width.  NT: tokens per tile, at most.  Narrow
+// tiles, for few rows per expert, leave room for ten stages and for accumulators ahead of the
+// workers: there the weights' stream from HBM is all that counts, and nothing may pause it.
+template <bool E8, int NT>
+struct Plan {
+    // e8m0: 4 scale warps (one per TMEM lane quadrant); f32: 2, and the wide tile's accumulators need
+    // the registers of a smaller block
     static constexpr int SCALE0 = E8 ? 4 : 2, SCALERS = E8 ? 4 : 2, WORK0 = SCALE0 + SCALERS;
     static constexpr int THREADS = 32 * (WORK0 + WORKERS);
+    static constexpr bool SPLIT = !E8 && NT == 256;      // workers take registers from the other roles
+    static constexpr int ABYTES = 128 * 128, BBYTES = NT / 2 * 128, STAGE = ABYTES + BBYTES;
+    static constexpr int STAGES = NT == 256 ? 6 : 10;
+    // TMEM: sums of whole tiles (e8m0) and two groups of scale factors, or products of K steps (f32)
+    static constexpr int NACC = E8 ? (NT == 256 ? 1 : 4) : 512 / NT;
+    static constexpr int SFB = NT / 32 < 4 ? 4 : NT / 32;  // columns of a K step's token scale factors
+    static constexpr uint32_t COL_SFA = 256, COL_SFB = COL_SFA + 2 * SGRP * 4;
+    static constexpr int NBAR = 2 * STAGES + 2 * NACC + 5;
+    static constexpr int OFF_S = STAGES * STAGE;         // scales: [2][SGRP][NT] f32 or [2][NT] x 8 bytes
+    static constexpr int OFF_LO = OFF_S + 2 * SGRP * NT * 4;  // [MAX_E] first row
+    static constexpr int OFF_CNT = OFF_LO + MAX_E * 4;   // [MAX_E] rows
+    static constexpr int OFF_T = OFF_CNT + MAX_E * 4;    // [MAX_E + 1] first token tile
+    static constexpr int OFF_BAR = OFF_T + (MAX_E + 4) * 4;
+    static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
+    static_assert(SMEM <= SMEM_MAX && OFF_BAR % 8 == 0, "shared memory");
+    static_assert(!E8 || (NACC * NT <= 256 && COL_SFB + 2 * SGRP * SFB <= 512), "tensor memory");
 };
 
 struct Args {
@@ -245,29 +252,33 @@ __device__ __forceinline__ int source_row(const Args &p, int r, bool &valid) {
     return valid ? s : 0;
 }
 
-template <bool E8>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 1)
+template <bool E8, int NT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREADS, 1)
     k_grouped_fp8(const __grid_constant__ Args p) {
-    using L = Roles<E8>;
+    using L = Plan<E8, NT>;
+    constexpr int STAGES = L::STAGES, STAGE = L::STAGE, ABYTES = L::ABYTES, NACC = L::NACC, HALF = NT / 2;
+    constexpr uint32_t COL_SFA = L::COL_SFA, COL_SFB = L::COL_SFB;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bar = reinterpret_cast<uint64_t *>(base + OFF_BAR);
+    uint64_t *bar = reinterpret_cast<uint64_t *>(base + L::OFF_BAR);
     // full, ready-for-MMA and freed accumulators live in the leader; empty, acc_ready in both
-    uint64_t *full = bar, *empty = bar + STAGES, *acc_ready = empty + STAGES, *acc_free = acc_ready + 2;
-    uint64_t *sf_full = acc_free + 2, *sf_empty = sf_full + 2, *fin = sf_empty + 2;
-    uint32_t *tmem_base = reinterpret_cast<uint32_t *>(bar + NBAR);
+    uint64_t *full = bar, *empty = bar + STAGES, *acc_ready = empty + STAGES, *acc_free = acc_ready + NACC;
+    uint64_t *sf_full = acc_free + NACC, *sf_empty = sf_full + 2, *fin = sf_empty + 2;
+    uint32_t *tmem_base = reinterpret_cast<uint32_t *>(bar + L::NBAR);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_base + 1);
-    int *lo = reinterpret_cast<int *>(base + OFF_LO), *cnt = reinterpret_cast<int *>(base + OFF_CNT);
-    int *first = reinterpret_cast<int *>(base + OFF_T);
+    int *lo = reinterpret_cast<int *>(base + L::OFF_LO), *cnt = reinterpret_cast<int *>(base + L::OFF_CNT);
+    int *first = reinterpret_cast<int *>(base + L::OFF_T);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int nks = p.K / 128, nn = (p.N + 255) / 256, nb = (p.N + 127) / 128;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < NACC; ++j) {
             mbar_init(acc_ready + j, 1);
             mbar_init(acc_free + j, 2 * WORKERS);
+        }
+        for (int j = 0; j < 2; ++j) {
             mbar_init(sf_full + j, E8 ? 2 * L::SCALERS : L::SCALERS);
             mbar_init(sf_empty + j, E8 ? 1 : WORKERS);
         }
@@ -313,7 +324,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
     Tile t;
 
     if (warp == W_PROD) {
-        if constexpr (!E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         int gs = 0;
         bool ok = true;
         while (ok && walk.next(t)) {
@@ -358,26 +369,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
             while (clock64() - t0 < 8000000) {}
         }
     } else if (warp == W_MMA) {
-        if constexpr (!E8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // The whole warp walks the loop and one elected lane issues, so that descriptors stay in
         // uniform registers (a loop run by one lane alone moves every operand there by itself:
         // 850 cycles per K step, more than its product takes).
         if (rank == 0) {
             const bool leader = elect_one();
             const uint64_t ad0 = smem_desc_sw128(base), bd0 = smem_desc_sw128(base + ABYTES);
-            int st = 0, gs = 0, sg = 0, ti = 0;
-            uint32_t phase = 0;
+            int st = 0, sg = 0, acc = 0;      // stage, group of scales, accumulator
+            uint32_t phase = 0, aphase = 1;   // (a fresh barrier passes a wait for the phase before)
             bool ok = true;
-            for (; ok && walk.next(t); ++ti) {
+            while (ok && walk.next(t)) {
                 const int width = __shfl_sync(0xffffffffu, t.width, 0);
-                if (E8) ok = ti < 1 || twait(acc_free, (ti - 1) & 1, abort, p.limit);
+                if (E8) ok = twait(acc_free + acc, aphase, abort, p.limit);
                 if (!__all_sync(0xffffffffu, ok)) break;
-                for (int ks = 0; ks < nks; ++ks, ++gs) {
-                    const int g = ks % SGRP, b = sg & 1, ab = gs & 1;
+                for (int ks = 0; ks < nks; ++ks) {
+                    const int g = ks % SGRP, b = sg & 1;
                     if (E8) {
                         if (g == 0) ok = twait(sf_full + b, (sg / 2) & 1, abort, p.limit);
                     } else {
-                        ok = gs < 2 || twait(acc_free + ab, (gs / 2 - 1) & 1, abort, p.limit);
+                        ok = twait(acc_free + acc, aphase, abort, p.limit);
                     }
                     ok = ok && twait(full + st, phase, abort, p.limit);
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -387,22 +398,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
                         if (E8) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                mma_mx(tm, ad + 2 * j, bd + 2 * j, idesc_mx(width, j), tm + COL_SFA + 4 * (SGRP * b + g),
-                                       tm + COL_SFB + 8 * (SGRP * b + g), (ks | j) != 0);
+                                mma_mx(tm + NT * acc, ad + 2 * j, bd + 2 * j, idesc_mx(width, j), tm + COL_SFA + 4 * (SGRP * b + g),
+                                       tm + COL_SFB + L::SFB * (SGRP * b + g), (ks | j) != 0);
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) mma_f8(tm + NT * ab, ad + 2 * j, bd + 2 * j, idesc_f8(width), j != 0);
+                            for (int j = 0; j < 4; ++j) mma_f8(tm + NT * acc, ad + 2 * j, bd + 2 * j, idesc_f8(width), j != 0);
                         }
                         commit2(empty + st);
-                        if (!E8) commit2(acc_ready + ab);
+                        if (!E8) commit2(acc_ready + acc);
                         if (E8 && (g == SGRP - 1 || ks == nks - 1)) commit2(sf_empty + b);
                     }
                     __syncwarp();
                     if (g == SGRP - 1 || ks == nks - 1) ++sg;
                     if (++st == STAGES) { st = 0; phase ^= 1; }
+                    if (!E8 && ++acc == NACC) { acc = 0; aphase ^= 1; }
                 }
-                if (E8 && ok && leader) commit2(acc_ready);
-                __syncwarp();
+                if (E8) {
+                    if (ok && leader) commit2(acc_ready + acc);
+                    __syncwarp();
+                    if (++acc == NACC) { acc = 0; aphase ^= 1; }
+                }
             }
             if (leader) commit2(fin, 1);  // TMEM and the peer's operands go only when every MMA is done
             twait(fin, 0, abort, kWaitLimitCycles);
@@ -413,7 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
         if constexpr (E8) {
             // Scale factors into TMEM.  Every lane quadrant holds all of them, so each warp writes
             // its own copy; the global loads are shared through shared memory.
-            uint2 *sb = reinterpret_cast<uint2 *>(base + OFF_S);
+            uint2 *sb = reinterpret_cast<uint2 *>(base + L::OFF_S);
             const int i = threadIdx.x - 32 * L::SCALE0;  // this thread loads tokens i and i + 128
             const uint32_t lanes = tm + ((uint32_t)(32 * (warp & 3)) << 16);
             const uint8_t *as = (const uint8_t *)p.a_s, *ws = (const uint8_t *)p.w_s;
@@ -421,9 +436,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
             int sg = 0;
             bool ok = true;
             while (ok && walk.next(t)) {
-                size_t ai[2];
+                size_t ai[(NT + 127) / 128];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < (NT + 127) / 128; ++h) {
                     bool valid;
                     ai[h] = (size_t)source_row(p, t.r0 + min(i + 128 * h, t.nrow - 1), valid) * nks;
                 }
@@ -432,8 +447,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
                 for (int k0 = 0; k0 < nks; k0 += SGRP, ++sg) {
                     const int b = sg & 1;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (128 * h >= t.width) break;
+                    for (int h = 0; h < (NT + 127) / 128; ++h) {
+                        if (i + 128 * h >= t.width) break;
                         uint2 v = make_uint2(0, 0);
                         if (wide) {
                             v = __ldg(reinterpret_cast<const uint2 *>(as + ai[h] + k0));
@@ -460,7 +475,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
                         uint32_t f[NT / 32];
 #pragma unroll
                         for (int c = 0; c < NT / 32; ++c) f[c] = __byte_perm(g < 4 ? v[c].x : v[c].y, 0, 0x1111 * (g & 3));
-                        tmem_st8(lanes + COL_SFB + 8 * (SGRP * b + g), f);
+                        if constexpr (NT == 256) tmem_st8(lanes + COL_SFB + L::SFB * (SGRP * b + g), f);
+                        else tmem_st4(lanes + COL_SFB + L::SFB * (SGRP * b + g), f[0], f[1], f[0], f[1]);
                         tmem_st4(lanes + COL_SFA + 4 * (SGRP * b + g), wb[g], wb[g], wb[g], wb[g]);
                     }
                     tmem_wait_st();
@@ -472,15 +488,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
             for (int u = max(0, sg - 2); ok && u < sg; ++u) ok = twait(sf_empty + (u & 1), (u / 2) & 1, abort, p.limit);
         } else {
             // token scale x weight scale of each K step into shared memory
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-            float *sa = reinterpret_cast<float *>(base + OFF_S);
+            if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+            float *sa = reinterpret_cast<float *>(base + L::OFF_S);
             const int i = threadIdx.x - 32 * L::SCALE0;  // this thread: tokens i, i + 64, ...
             int sg = 0;
             bool ok = true;
             while (ok && walk.next(t)) {
-                size_t ai[4];
+                size_t ai[NT / 64];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
+                for (int h = 0; h < NT / 64; ++h) {
                     bool valid;
                     ai[h] = (size_t)source_row(p, t.r0 + min(i + 64 * h, t.nrow - 1), valid) * nks;
                 }
@@ -490,18 +506,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
                     if (sg >= 2) ok = twait(sf_empty + b, (sg / 2 - 1) & 1, abort, p.limit);
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     // all loads of the group before the first use: one trip to memory, not one per step
-                    float w[SGRP], v[4][SGRP];
+                    float w[SGRP], v[NT / 64][SGRP];
 #pragma unroll
                     for (int g = 0; g < SGRP; ++g) {
                         const int k = min(k0 + g, nks - 1);
                         w[g] = scale_at(p.w_s, p.w_f32, wi + k);
 #pragma unroll
-                        for (int h = 0; h < 4; ++h) v[h][g] = 64 * h < t.width ? scale_at(p.a_s, p.a_f32, ai[h] + k) : 0.f;
+                        for (int h = 0; h < NT / 64; ++h) v[h][g] = 64 * h < t.width ? scale_at(p.a_s, p.a_f32, ai[h] + k) : 0.f;
                     }
 #pragma unroll
                     for (int g = 0; g < SGRP; ++g)
 #pragma unroll
-                        for (int h = 0; h < 4; ++h)
+                        for (int h = 0; h < NT / 64; ++h)
                             if (64 * h < t.width) sa[(b * SGRP + g) * NT + i + 64 * h] = v[h][g] * w[g];
                     __syncwarp();
                     if (lane == 0) mbar_arrive(sf_full + b);
@@ -509,35 +525,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
             }
         }
     } else {
-        // workers: warp (q, half) takes the 32 weight rows of TMEM lane quadrant q and 128 of the
-        // tile's tokens
-        if constexpr (!E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // workers: warp (q, half) takes the 32 weight rows of TMEM lane quadrant q and half of the
+        // widest tile's tokens
+        if constexpr (L::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int q = warp & 3, half = (warp - L::WORK0) >> 2;
-        const uint32_t col = tm + ((uint32_t)(32 * q) << 16) + 128 * half;
-        const float *sa = reinterpret_cast<const float *>(base + OFF_S) + 128 * half;
-        int gs = 0, sg = 0, ti = 0;
+        const uint32_t col = tm + ((uint32_t)(32 * q) << 16) + HALF * half;
+        const float *sa = reinterpret_cast<const float *>(base + L::OFF_S) + HALF * half;
+        int sg = 0, acc = 0;
+        uint32_t aphase = 0;
         bool ok = true;
-        for (; ok && walk.next(t); ++ti) {
-            const int mine = min(t.nrow - 128 * half, 128);  // tokens of this warp that are stored
-            uint32_t keep[4];  // those whose row of `a` exists; the others' results are zero
+        while (ok && walk.next(t)) {
+            const int mine = min(t.nrow - HALF * half, HALF);  // tokens of this warp that are stored
+            uint32_t keep[HALF / 32];  // those whose row of `a` exists; the others' results are zero
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < HALF / 32; ++c) {
                 bool valid = true;
-                if (32 * c + lane < mine) source_row(p, t.r0 + 128 * half + 32 * c + lane, valid);
+                if (32 * c + lane < mine) source_row(p, t.r0 + HALF * half + 32 * c + lane, valid);
                 keep[c] = __ballot_sync(0xffffffffu, valid);
             }
             const int n = t.n0 + 128 * rank + 32 * q + lane;
-            __nv_bfloat16 *o = p.out + (size_t)(t.r0 + 128 * half) * p.N + n;
+            __nv_bfloat16 *o = p.out + (size_t)(t.r0 + HALF * half) * p.N + n;
             if constexpr (E8) {
-                ok = twait(acc_ready, ti & 1, abort, p.limit);
+                ok = twait(acc_ready + acc, aphase, abort, p.limit);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 fence_after_sync();
-                __nv_bfloat162 y[64];
+                __nv_bfloat162 y[HALF / 2];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (128 * half + 32 * c >= t.width) break;
+                for (int c = 0; c < HALF / 32; ++c) {
+                    if (HALF * half + 32 * c >= t.width) break;
                     uint32_t v[32];
-                    tmem_ld32(col + 32 * c, v);
+                    tmem_ld32(col + NT * acc + 32 * c, v);
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -545,55 +562,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Roles<E8>::THREADS, 
                 }
                 fence_before_sync();
                 __syncwarp();
-                if (lane == 0) arrive_at(leader_addr(acc_free));
+                if (lane == 0) arrive_at(leader_addr(acc_free + acc));
+                if (++acc == NACC) { acc = 0; aphase ^= 1; }
                 if (n < p.N) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
+                    for (int j = 0; j < HALF; ++j)
                         if (j < mine)
                             o[(size_t)j * p.N] = !(keep[j / 32] >> (j % 32) & 1) ? __float2bfloat16_rn(0.f)
                                                  : j & 1                        ? __high2bfloat16(y[j / 2])
                                                                                 : __low2bfloat16(y[j / 2]);
                 }
             } else {
-                float acc[128];
+                float sum[HALF];
 #pragma unroll
-                for (int j = 0; j < 128; ++j) acc[j] = 0.f;
-                for (int ks = 0; ks < nks; ++ks, ++gs) {
-                    const int g = ks % SGRP, b = sg & 1, ab = gs & 1;
+                for (int j = 0; j < HALF; ++j) sum[j] = 0.f;
+                for (int ks = 0; ks < nks; ++ks) {
+                    const int g = ks % SGRP, b = sg & 1;
                     if (g == 0) ok = twait(sf_full + b, (sg / 2) & 1, abort, p.limit);
-                    ok = ok && twait(acc_ready + ab, (gs / 2) & 1, abort, p.limit);
+                    ok = ok && twait(acc_ready + acc, aphase, abort, p.limit);
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     fence_after_sync();
                     const float *s = sa + (b * SGRP + g) * NT;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (128 * half + 32 * c < t.width) {
+                    for (int c = 0; c < HALF / 32; ++c) {
+                        if (HALF * half + 32 * c < t.width) {
                             uint32_t v[32];
-                            tmem_ld32(col + NT * ab + 32 * c, v);
+                            tmem_ld32(col + NT * acc + 32 * c, v);
                             tmem_wait_ld();
 #pragma unroll
                             for (int j = 0; j < 32; j += 4) {
                                 const float4 f = *reinterpret_cast<const float4 *>(s + 32 * c + j);
-                                acc[32 * c + j] += f.x * __uint_as_float(v[j]);
-                                acc[32 * c + j + 1] += f.y * __uint_as_float(v[j + 1]);
-                                acc[32 * c + j + 2] += f.z * __uint_as_float(v[j + 2]);
-                                acc[32 * c + j + 3] += f.w * __uint_as_float(v[j + 3]);
+                                sum[32 * c + j] += f.x * __uint_as_float(v[j]);
+                                sum[32 * c + j + 1] += f.y * __uint_as_float(v[j + 1]);
+                                sum[32 * c + j + 2] += f.z * __uint_as_float(v[j + 2]);
+                                sum[32 * c + j + 3] += f.w * __uint_as_float(v[j + 3]);
                             }
                         }
                     }
                     fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
-                        arrive_at(leader_addr(acc_free + ab));
+                        arrive_at(leader_addr(acc_free + acc));
                         if (g == SGRP - 1 || ks == nks - 1) mbar_arrive(sf_empty + b);
                     }
                     if (g == SGRP - 1 || ks == nks - 1) ++sg;
+                    if (++acc == NACC) { acc = 0; aphase ^= 1; }
                 }
                 if (!ok) break;
                 if (n < p.N) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
-                        if (j < mine) o[(size_t)j * p.N] = __float2bfloat16_rn(keep[j / 32] >> (j % 32) & 1 ? acc[j] : 0.f);
+                    for (int j = 0; j < HALF; ++j)
+                        if (j < mine) o[(size_t)j * p.N] = __float2bfloat16_rn(keep[j / 32] >> (j % 32) & 1 ? sum[j] : 0.f);
                 }
             }
         }
@@ -647,6 +666,16 @@ int tensor_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t K, uint
     return WF_OK;
 }
 
+template <bool E8, int NT>
+cudaError_t launch(const Args &p, int sms, cudaStream_t st) {
+    using L = Plan<E8, NT>;
+    cudaError_t e = cudaFuncSetAttribute(k_grouped_fp8<E8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = ((int64_t)p.R / NT + (p.E < p.R ? p.E : p.R)) * ((p.N + 255) / 256);
+    k_grouped_fp8<E8, NT><<<2 * (unsigned)(tiles < sms / 2 ? tiles : sms / 2), L::THREADS, L::SMEM, st>>>(p);
+    return cudaSuccess;
+}
+
 }  // namespace grp
 }  // namespace wf
 
@@ -657,7 +686,7 @@ extern "C" {
 
 size_t wf_grouped_fp8_workspace_bytes(int32_t row_list, int64_t R, int32_t E, int64_t K) {
     if (R <= 0 || R > (1 << 30) || E <= 0 || E > wf::grp::MAX_E || K <= 0 || K > (1 << 20)) return 0;
-    return row_list && R > (int64_t)E * wf::grp::GATHER_ROWS ? (size_t)R * K : 0;
+    return row_list && R > (int64_t)E * wf::grp::FEW ? (size_t)R * K : 0;
 }
 
 int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, const void *w, const void *w_s,
@@ -679,7 +708,7 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
     // four rows a copy straight from a.  The TMA unit takes about 80 cycles for a four-row copy, so up
     // to 32 rows of a CTA (a tile of 64) hide behind the 128 weight rows of a K step (about 700 cycles of
     // its share of HBM), and 128 take four times as long as their product.
-    const bool pack = rows && R > (int64_t)E * wf::grp::GATHER_ROWS;
+    const bool pack = rows && R > (int64_t)E * wf::grp::FEW;
     if (pack) {
         if (!workspace || workspace_bytes < (size_t)R * K) return fail(WF_E_ARG, "workspace too small (see wf_grouped_fp8_workspace_bytes)");
         if ((uintptr_t)workspace % 16) return fail(WF_E_ARG, "workspace must be 16-byte aligned");
@@ -699,12 +728,7 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
     p.a_f32 = a_scale_kind == WF_SCALE_F32; p.w_f32 = w_scale_kind == WF_SCALE_F32;
     const int sms = wf::host::sm_count();
     if (sms <= 0) return fail(WF_E_CUDA, "no CUDA device");
-    const int64_t tiles = (R / wf::grp::NT + (E < R ? E : R)) * ((N + 255) / 256);
-    const unsigned grid = 2 * (unsigned)(tiles < sms / 2 ? tiles : sms / 2);
-    const bool e8 = !p.a_f32 && !p.w_f32;
-    const void *k = e8 ? (const void *)wf::grp::k_grouped_fp8<true> : (const void *)wf::grp::k_grouped_fp8<false>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, wf::grp::SMEM);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(grouped_fp8_gemm)");
+    const bool e8 = !p.a_f32 && !p.w_f32, few = R <= (int64_t)E * wf::grp::FEW;
     cudaStream_t st = (cudaStream_t)stream;
     if (pack) {
         const int64_t steps = R * (K / 16) / wf::grp::PACK_STEP + 1;
@@ -712,8 +736,9 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
             (const uint4 *)a, rows, offsets, (uint4 *)workspace, E, (int)M, (int)R, (int)(K / 16));
         wf::host::counted();
     }
-    if (e8) wf::grp::k_grouped_fp8<true><<<grid, wf::grp::Roles<true>::THREADS, wf::grp::SMEM, st>>>(p);
-    else wf::grp::k_grouped_fp8<false><<<grid, wf::grp::Roles<false>::THREADS, wf::grp::SMEM, st>>>(p);
+    cudaError_t e = e8 ? (few ? wf::grp::launch<true, 64>(p, sms, st) : wf::grp::launch<true, 256>(p, sms, st))
+                       : (few ? wf::grp::launch<false, 64>(p, sms, st) : wf::grp::launch<false, 256>(p, sms, st));
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(grouped_fp8_gemm)");
     wf::host::counted();
     e = cudaGetLastError();
     return e == cudaSuccess ? WF_OK : cuda_fail(e, "grouped_fp8_gemm launch");

@@ -188,6 +188,8 @@ struct RouteArgs {
     long long T;
     double scale;
     int E, k, G, keep, bf16, score, top2, renorm;
+    int per, part;   // experts per group, log2 of the lanes that share a group
+    uint32_t magic;  // e * magic >> 20 = e / per for e < 512
 };
 
 // doubles in an order that unsigned comparison keeps; 0 is below every value, NaN above
@@ -213,10 +215,23 @@ __device__ __forceinline__ double score64(double z, int score) {
     return sqrt((z > 0 ? z : 0.0) + log1p(exp(-fabs(z))));
 }
 
-// The whole choice in 64 bits; lane j < k returns the expert of slot j in my_idx (-1: none) and its score.
+__device__ __forceinline__ float logit_at(const RouteArgs &p, long long i) {
+    return p.bf16 ? __bfloat162float(((const __nv_bfloat16 *)p.logits)[i]) : __ldg((const float *)p.logits + i);
+}
+
+struct Pick {
+    int expert;    // -1: none
+    double score;
+};
+
+// The whole choice of token t in 64 bits: lane j < k returns slot j.  Out of line, and with the
+// logits read anew, so that the common path keeps its registers.
 template <int N>
-__device__ __noinline__ double route64(const RouteArgs &p, const float (&zf)[N], int &my_idx) {
+__device__ __noinline__ Pick route64(const RouteArgs &p, long long t) {
     const int lane = threadIdx.x & 31;
+    float zf[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) zf[i] = lane + 32 * i < p.E ? logit_at(p, t * p.E + lane + 32 * i) : -CUDART_INF_F;
     double s[N];
     unsigned long long key[N];
     double top = -CUDART_INF;
@@ -295,8 +310,7 @@ __device__ __noinline__ double route64(const RouteArgs &p, const float (&zf)[N],
             if (e < p.E && !(kept >> (e / per) & 1)) key[i] = 0;
         }
     }
-    my_idx = -1;
-    double mine = 0.0;
+    Pick mine = {-1, 0.0};
     for (int j = 0; j < p.k; ++j) {
         unsigned long long a = 0;
         double sa = 0.0;
@@ -311,12 +325,15 @@ __device__ __noinline__ double route64(const RouteArgs &p, const float (&zf)[N],
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if ((uint32_t)(lane + 32 * i) == best) key[i] = 0;
-        if (lane == j) {
-            my_idx = (int)best;
-            mine = sb;
-        }
+        if (lane == j) mine = {(int)best, sb};
     }
     return mine;
+}
+
+// sel of expert e of token t in 64 bits
+__device__ __noinline__ double sel64(const RouteArgs &p, long long t, int e) {
+    const double s = score64((double)logit_at(p, t * p.E + e), p.score);
+    return p.bias ? s + (double)__ldg(p.bias + e) : s;
 }
 
 // 32-bit keys: order kept under unsigned comparison, 0 below every value
@@ -328,47 +345,89 @@ __device__ __forceinline__ float value32(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// The groups kept, one bit each, by 64-bit values of their best experts (32-bit keys a and b of
+// group grp in its leader lane); 0 where a third expert is too near to tell which two are best.
+__device__ __noinline__ uint32_t groups64(const RouteArgs &p, long long t, const uint32_t *sm, uint32_t a, uint32_t b, int grp,
+                                          bool leader, float gap0) {
+    const int lane = threadIdx.x & 31;
+    int ea = -1, eb = -1;
+    uint32_t c = 0;
+    if (leader) {
+        for (int j = 0; j < p.per; ++j) {
+            const uint32_t v = sm[grp * p.per + j];
+            if (v == a && ea < 0) ea = grp * p.per + j;
+            else if (v == b && eb < 0) eb = grp * p.per + j;
+            else c = max(c, v);
+        }
+    }
+    const float edge = p.top2 ? value32(b) : value32(a);
+    if (__any_sync(0xffffffffu, leader && c && !(edge - value32(c) > gap0 + fmaxf(fabsf(edge), fabsf(value32(c))) * 0x1p-17f)))
+        return 0;
+    const double xa = sel64(p, t, max(ea, 0)), xb = sel64(p, t, max(eb, 0));
+    unsigned long long mine = 0;
+    if (leader && a) mine = order_key(!b ? xa : p.top2 ? xa + xb : fmax(xa, xb));
+    uint32_t kept = 0;
+    for (int j = 0; j < p.keep; ++j) {
+        const unsigned long long m = warp_max(mine);
+        if (!m) break;
+        const int who = __ffs(__ballot_sync(0xffffffffu, mine == m)) - 1;
+        kept |= 1u << __shfl_sync(0xffffffffu, grp, who);
+        if (lane == who) mine = 0;
+    }
+    return kept;
+}
+
 // The choice screened in 32 bits.  A 32-bit score is off by less than 2^-21 of itself (expf and
-// log1pf to 2 ulp, an addition, a division or a square root) and sel by half an ulp more, so two
-// values further apart than `gap` are in the right order; where any decision of the row (a slot
-// against the next, the last group kept against the first dropped) is closer than that, or the
-// row has NaN, +infinity or too few experts, the row is left to route64.  Returns whether all
-// decisions stand; lane j < k has the expert of slot j.
+// log1pf to 2 ulp, an addition, a reciprocal or a square root) and sel by half an ulp more; its key
+// gives up its 4 lowest bits (2^-19 of sel) to the place of the expert in its lane, so one
+// reduction finds a winner and where it sits.  Two values further apart than `gap` are in the
+// right order; a winner closer than that to the one before it (1.2 % of rows of 256 normal logits)
+// is put in its place by the 64-bit values of the winners so far, one evaluation in all lanes at
+// once, and so is a choice of groups (0.1 % of rows of 8 groups).  Rows with NaN, +infinity or too
+// few experts and long runs of equal values are left to route64, which takes several times as
+// long (and a launch as long as its slowest row: settling rows here took 8191 x 256 in 8 groups
+// from 30 to 19 us).  Returns whether the row was settled; lane j < k has the expert of slot j.
 template <int N>
-__device__ __forceinline__ bool route32(const RouteArgs &p, const float (&z)[N], uint32_t *sm, int &my_idx) {
+__device__ __forceinline__ bool route32(const RouteArgs &p, long long t, const float (&z)[N], const float (&bias)[N],
+                                        uint32_t *sm, int &my_idx) {
+    static_assert(N <= 16, "4 bits for the place in the lane");
     const int lane = threadIdx.x & 31;
     uint32_t key[N];
-    float smax = 0.f;
-    bool odd = false;
+    float smax = 0.f, all = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int e = lane + 32 * i;
-        odd |= !(z[i] < CUDART_INF_F);
         float sc;
-        if (p.score == WF_SCORE_SIGMOID) sc = __frcp_rn(1.0f + expf(-z[i]));
-        else sc = __fsqrt_rn(fmaxf(z[i], 0.f) + log1pf(expf(-fabsf(z[i]))));
+        if (p.score == WF_SCORE_SIGMOID) {
+            const float d = 1.0f + expf(-z[i]);
+            asm("rcp.approx.f32 %0, %1;" : "=f"(sc) : "f"(d));
+        } else {
+            sc = __fsqrt_rn(fmaxf(z[i], 0.f) + log1pf(expf(-fabsf(z[i]))));
+        }
+        const float sel = sc + bias[i];
         smax = fmaxf(smax, sc);
-        const float sel = p.bias && e < p.E ? sc + __ldg(p.bias + e) : sc;
-        odd |= !(sel < CUDART_INF_F);
-        key[i] = z[i] == -CUDART_INF_F || sel == -CUDART_INF_F ? 0u : key32(sel + 0.0f);
+        all = max_nan(all, max_nan(z[i], sel));
+        key[i] = z[i] == -CUDART_INF_F || sel == -CUDART_INF_F ? 0u : (key32(sel) & ~15u) | i;
     }
-    if (__any_sync(0xffffffffu, odd)) return false;
+    if (__any_sync(0xffffffffu, !(all < CUDART_INF_F))) return false;
     smax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)));  // scores are not negative
     if (smax < 0x1p-40f) return false;  // subnormal steps of expf: the bound above does not hold
     const float gap0 = smax * 0x1p-18f;
     if (p.G > 1) {
         // 2^w lanes per group: each takes every 2^w-th expert of it, then their best two are merged
-        const int per = p.E / p.G, w = 31 - __clz(32 / p.G), sub = lane & ((1 << w) - 1), grp = lane >> w;
+        const int per = p.per, w = p.part, sub = lane & ((1 << w) - 1), grp = lane >> w;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (lane + 32 * i < p.E) sm[lane + 32 * i] = key[i];
+        for (int i = 0; i < N; ++i) sm[lane + 32 * i] = key[i];
         __syncwarp();
         uint32_t a = 0, b = 0;
         if (grp < p.G) {
-            for (int j = sub; j < per; j += 1 << w) {
-                const uint32_t v = sm[grp * per + j];
+            const int n = (per - sub + (1 << w) - 1) >> w;
+            const uint32_t *g = sm + grp * per + sub;
+            int q = grp < n ? grp : 0;  // groups start apart: their lanes read other banks
+            for (int j = 0; j < n; ++j) {
+                const uint32_t v = g[q << w];
                 b = max(b, min(a, v));
                 a = max(a, v);
+                if (++q == n) q = 0;
             }
         }
         for (int o = 1; o < 1 << w; o <<= 1) {
@@ -382,7 +441,7 @@ __device__ __forceinline__ bool route32(const RouteArgs &p, const float (&z)[N],
         uint32_t mine = a;
         if (p.top2 && b) {
             const float v = value32(a) + value32(b);
-            mine = v > -CUDART_INF_F ? key32(v + 0.0f) : 0u;
+            mine = v > -CUDART_INF_F ? key32(v) : 0u;
         }
         if (sub) mine = 0;
         uint32_t kept = 0, m = 0;
@@ -394,74 +453,72 @@ __device__ __forceinline__ bool route32(const RouteArgs &p, const float (&z)[N],
             if (lane == who) mine = 0;
         }
         const uint32_t next = __reduce_max_sync(0xffffffffu, mine);
-        if (next) {
-            if (!(value32(m) - value32(next) > 2 * gap0 + mag * 0x1p-18f)) return false;
+        if (next && !(value32(m) - value32(next) > 2 * gap0 + mag * 0x1p-16f)) {
+            kept = groups64(p, t, sm, a, b, grp, sub == 0 && grp < p.G, gap0);
+            if (!kept) return false;
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = lane + 32 * i;
-            if (e < p.E && !(kept >> (e / per) & 1)) key[i] = 0;
-        }
+        for (int i = 0; i < N; ++i)
+            if (!(kept >> ((lane + 32 * i) * p.magic >> 20) & 1)) key[i] = 0;  // (past E: 0 already)
     }
     my_idx = -1;
-    float last = 0.f;
-    for (int j = 0; j <= p.k; ++j) {
+    float last = 0.f, kth = 0.f;
+    for (int j = 0; j < p.k + 8; ++j) {
         uint32_t a = 0;
-        int e = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (key[i] > a) { a = key[i]; e = lane + 32 * i; }
+        for (int i = 0; i < N; ++i) a = max(a, key[i]);
         const uint32_t m = __reduce_max_sync(0xffffffffu, a);
-        if (!m) return j == p.k;
+        if (!m) return j >= p.k;
         const float v = value32(m);
-        if (j > 0 && !(last - v > gap0 + fmaxf(fabsf(last), fabsf(v)) * 0x1p-18f)) return false;
-        if (j == p.k) break;
-        last = v;
+        // the slots hold the k best so far: what is left cannot pass the k-th by its error
+        if (j >= p.k && kth - v > gap0 + fmaxf(fabsf(kth), fabsf(v)) * 0x1p-17f) return true;
         const int who = __ffs(__ballot_sync(0xffffffffu, a == m)) - 1;
-        const int best = __shfl_sync(0xffffffffu, e, who);
+        const int e = who + 32 * (int)(m & 15);
+        const uint32_t gone = lane == who ? m : 0u;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (lane + 32 * i == best) key[i] = 0;
-        if (lane == j) my_idx = best;
+            if (key[i] == gone) key[i] = 0;
+        if (j == 0 || last - v > gap0 + fmaxf(fabsf(last), fabsf(v)) * 0x1p-17f) {
+            if (lane == j) my_idx = e;
+        } else {
+            const int have = min(j, p.k), mine = lane < have ? my_idx : e;
+            const double x = sel64(p, t, mine), xe = __shfl_sync(0xffffffffu, x, 31);
+            const int rank = __popc(__ballot_sync(0xffffffffu, lane < have && (x > xe || (x == xe && mine < e))));
+            const int below = __shfl_up_sync(0xffffffffu, my_idx, 1);
+            if (lane < p.k) my_idx = lane == rank ? e : lane > rank && lane <= have ? below : my_idx;
+        }
+        last = v;
+        if (j == p.k - 1) kth = v;
     }
-    return true;
+    return false;
 }
 
 template <int N>  // experts per lane
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route_topk(const __grid_constant__ RouteArgs p) {
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, N <= 8 ? 8 : 4) k_route_topk(const __grid_constant__ RouteArgs p) {
     __shared__ uint32_t sm[ROUTE_WARPS][32 * N];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long t = (long long)blockIdx.x * ROUTE_WARPS + warp;
     if (t >= p.T) return;
-    float z[N];
+    float z[N], bias[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int e = lane + 32 * i;
-        z[i] = -CUDART_INF_F;
-        if (e < p.E)
-            z[i] = p.bf16 ? __bfloat162float(((const __nv_bfloat16 *)p.logits)[t * p.E + e])
-                          : __ldg((const float *)p.logits + t * p.E + e);
+        z[i] = lane + 32 * i < p.E ? logit_at(p, t * p.E + lane + 32 * i) : -CUDART_INF_F;
+        bias[i] = p.bias && lane + 32 * i < p.E ? __ldg(p.bias + lane + 32 * i) : 0.f;
     }
-    int idx = -1;
-    double s;
+    Pick pick;
     // softmax weights need the row's sum in 64 bits anyway
-    if (p.score != WF_SCORE_SOFTMAX && route32<N>(p, z, sm[warp], idx)) {
-        const long long at = t * p.E + max(idx, 0);
-        s = idx < 0 ? 0.0
-                    : score64(p.bf16 ? (double)__bfloat162float(((const __nv_bfloat16 *)p.logits)[at])
-                                     : (double)__ldg((const float *)p.logits + at),
-                              p.score);
-    } else {
-        s = route64<N>(p, z, idx);
-    }
+    if (p.score != WF_SCORE_SOFTMAX && route32<N>(p, t, z, bias, sm[warp], pick.expert))
+        pick.score = pick.expert < 0 ? 0.0 : score64((double)logit_at(p, t * p.E + pick.expert), p.score);
+    else
+        pick = route64<N>(p, t);
     if (p.renorm) {
         double sum = 0.0;  // the same order in every lane
-        for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, s, j);
-        s = sum == 0.0 ? 0.0 : s / sum;
+        for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, pick.score, j);
+        pick.score = sum == 0.0 ? 0.0 : pick.score / sum;
     }
     if (lane < p.k) {
-        p.w[t * p.k + lane] = (float)(idx < 0 ? 0.0 : s * p.scale);
-        p.idx[t * p.k + lane] = idx;
+        p.w[t * p.k + lane] = (float)(pick.expert < 0 ? 0.0 : pick.score * p.scale);
+        p.idx[t * p.k + lane] = pick.expert;
     }
 }
 
@@ -767,6 +824,10 @@ int wf_route_topk(const void *logits, int32_t logits_bf16, const float *bias, in
     p.T = T; p.scale = route_scale; p.E = E; p.k = topk; p.G = n_groups == topk_groups ? 1 : n_groups;
     p.keep = topk_groups; p.bf16 = logits_bf16 != 0; p.score = score_func; p.top2 = group_top2 != 0;
     p.renorm = renorm != 0;
+    p.per = E / n_groups;
+    p.magic = ((1u << 20) + p.per - 1) / p.per;
+    p.part = 0;
+    while (2 << p.part <= 32 / n_groups) ++p.part;
     const unsigned g = (unsigned)((T + ROUTE_WARPS - 1) / ROUTE_WARPS);
     cudaStream_t st = (cudaStream_t)stream;
     const int per = (E + 31) / 32;
