@@ -186,6 +186,14 @@ __device__ __forceinline__ void tma_load2(void *dst, const CUtensorMap *map, int
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
+// The same with an L2 policy.
+__device__ __forceinline__ void tma_load2_hint(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t bar, uint64_t pol) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar), "l"(pol)
+        : "memory");
+}
 // Four rows of the tensor map, 128 bytes each, to 512 consecutive (swizzled) bytes.
 __device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, int c0, int4 r, uint32_t bar) {
     asm volatile(
@@ -250,6 +258,12 @@ __device__ __forceinline__ int source_row(const Args &p, int r, bool &valid) {
     const int s = p.rows ? __ldg(p.rows + r) : r;
     valid = s >= 0 && s < p.M;
     return valid ? s : 0;
+}
+
+// Rows of the tile that CTA `rank` of the pair loads: in fours to gather, else in sixteens.
+__device__ __forceinline__ int rows_held(const Tile &t, int half, int rank, int gather) {
+    const int n = min(max(t.nrow - half * rank, 0), half);
+    return gather ? (n + 3) & ~3 : (n + 15) & ~15;
 }
 
 template <bool E8, int NT>
@@ -327,8 +341,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
         if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         int gs = 0;
         bool ok = true;
+        // Narrow tiles read most weights once, wide ones several times: evict-first took 1536 rows
+        // over 64 experts of 2048 x 1024 from 41.0 to 38.9 us and cost wide tiles 6 %.
+        const uint64_t pol = policy_evict_first();
         while (ok && walk.next(t)) {
-            const int half = t.width / 2;  // this CTA's tokens of the tile
+            // The pair's rows of the tile, half each; columns behind the tile's last row hold what
+            // the stage held before and are not stored.
+            const int half = t.width / 2, mine = rows_held(t, half, rank, p.gather);
+            const uint32_t bytes = 2 * ABYTES + 128 * (rows_held(t, half, 0, p.gather) + rows_held(t, half, 1, p.gather));
             int src[4];
             if (p.gather) {
 #pragma unroll
@@ -344,18 +364,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
                 uint8_t *dst = base + st * STAGE;
                 const uint32_t fb = leader_addr(full + st);
                 if (lane == 0) {
-                    if (rank == 0) mbar_arrive_expect_tx(full + st, 2 * (ABYTES + half * 128));
-                    tma_load2(dst, &p.tmW, ks * 128, t.e * p.N + t.n0 + 128 * rank, fb);
+                    if (rank == 0) mbar_arrive_expect_tx(full + st, bytes);
+                    if constexpr (NT == 256) tma_load2(dst, &p.tmW, ks * 128, t.e * p.N + t.n0 + 128 * rank, fb);
+                    else tma_load2_hint(dst, &p.tmW, ks * 128, t.e * p.N + t.n0 + 128 * rank, fb, pol);
                 }
                 __syncwarp();
                 if (p.gather) {
-                    if (4 * lane < half)
+                    if (4 * lane < mine)
                         tma_gather4(dst + ABYTES + lane * 512, &p.tmA[0], ks * 128, make_int4(src[0], src[1], src[2], src[3]), fb);
-                } else if (lane < 4 && half & 128 >> lane) {
-                    // half as a sum of boxes, one a lane: a copy costs the TMA unit about as much
-                    // whatever its height (boxes of 16 rows alone: 2091 against 3050 TFLOP/s for one
-                    // expert of 16384 rows, 4096 x 4096)
-                    const int at = half & ~(0xff >> lane);
+                } else if (lane < 4 && mine & 128 >> lane) {
+                    // a sum of boxes, one a lane: a copy costs the TMA unit about as much whatever its
+                    // height (boxes of 16 rows alone: 2091 against 3050 TFLOP/s for one expert of
+                    // 16384 rows, 4096 x 4096)
+                    const int at = mine & ~(0xff >> lane);
                     tma_load2(dst + ABYTES + at * 128, &p.tmA[lane], ks * 128, t.r0 + half * rank + at, fb);
                 }
             }
