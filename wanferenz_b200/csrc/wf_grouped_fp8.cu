@@ -19,6 +19,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/wfb200.h"
 #include "wf_host.h"
 #include "wf_ptx.cuh"
@@ -301,6 +303,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
         fence_mbar_init();
     }
     if (warp == W_MMA) tmem_alloc2(tmem_base, 512);
+    pdl_launch_dependents();
+    pdl_wait();
     // every expert's rows, clamped to the R rows there are, and its first token tile
     for (int e = threadIdx.x; e < p.E; e += L::THREADS) {
         const int a = min(max(p.offsets[e], 0), p.R), b = min(max(p.offsets[e + 1], 0), p.R);
@@ -651,6 +655,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
 constexpr int PACK_STEP = 4 * 256;
 __global__ void __launch_bounds__(256) k_pack_rows(const uint4 *a, const int *rows, const int *offsets, uint4 *out, int E,
                                                    int M, int R, int chunks) {
+    pdl_launch_dependents();
+    pdl_wait();
     // rows behind the last expert's are left out; the offsets need not rise
     int end = 0;
     for (int e = threadIdx.x; e <= E; e += 256) end = max(end, __ldg(offsets + e));
@@ -690,11 +696,19 @@ int tensor_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t K, uint
 template <bool E8, int NT>
 cudaError_t launch(const Args &p, int sms, cudaStream_t st) {
     using L = Plan<E8, NT>;
-    cudaError_t e = cudaFuncSetAttribute(k_grouped_fp8<E8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+    // once per device (the attribute is the function's, whichever thread sets it)
+    static std::atomic<uint64_t> ready{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(k_grouped_fp8<E8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
     const int64_t tiles = ((int64_t)p.R / NT + (p.E < p.R ? p.E : p.R)) * ((p.N + 255) / 256);
-    k_grouped_fp8<E8, NT><<<2 * (unsigned)(tiles < sms / 2 ? tiles : sms / 2), L::THREADS, L::SMEM, st>>>(p);
-    return cudaSuccess;
+    return host::launch_pdl(k_grouped_fp8<E8, NT>, dim3(2 * (unsigned)(tiles < sms / 2 ? tiles : sms / 2)), L::THREADS, L::SMEM, st, p);
 }
 
 }  // namespace grp
@@ -751,17 +765,15 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
     if (sms <= 0) return fail(WF_E_CUDA, "no CUDA device");
     const bool e8 = !p.a_f32 && !p.w_f32, few = R <= (int64_t)E * wf::grp::FEW;
     cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = cudaSuccess;
     if (pack) {
         const int64_t steps = R * (K / 16) / wf::grp::PACK_STEP + 1;
-        wf::grp::k_pack_rows<<<(unsigned)(steps < 8 * sms ? steps : 8 * sms), 256, 0, st>>>(
-            (const uint4 *)a, rows, offsets, (uint4 *)workspace, E, (int)M, (int)R, (int)(K / 16));
-        wf::host::counted();
+        e = wf::host::launch_pdl(wf::grp::k_pack_rows, dim3((unsigned)(steps < 8 * sms ? steps : 8 * sms)), 256, 0, st,
+                                 (const uint4 *)a, rows, offsets, (uint4 *)workspace, (int)E, (int)M, (int)R, (int)(K / 16));
     }
-    cudaError_t e = e8 ? (few ? wf::grp::launch<true, 64>(p, sms, st) : wf::grp::launch<true, 256>(p, sms, st))
-                       : (few ? wf::grp::launch<false, 64>(p, sms, st) : wf::grp::launch<false, 256>(p, sms, st));
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(grouped_fp8_gemm)");
-    wf::host::counted();
-    e = cudaGetLastError();
+    if (e == cudaSuccess)
+        e = e8 ? (few ? wf::grp::launch<true, 64>(p, sms, st) : wf::grp::launch<true, 256>(p, sms, st))
+               : (few ? wf::grp::launch<false, 64>(p, sms, st) : wf::grp::launch<false, 256>(p, sms, st));
     return e == cudaSuccess ? WF_OK : cuda_fail(e, "grouped_fp8_gemm launch");
 }
 

@@ -25,5 +25,24 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
 // cuTensorMapEncodeTiled through the runtime's driver entry point (NULL when unavailable).
 EncodeTiledFn encode_fn() noexcept;
 
+// Launches `kernel` so that it may start while the kernel before it on the stream drains
+// (programmatic dependent launch).  Every CTA of `kernel` executes griddepcontrol.wait before it
+// touches global memory, so the order of the stream holds for what it reads and writes.
+template <class... P, class... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    counted();
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace host
 }  // namespace wf

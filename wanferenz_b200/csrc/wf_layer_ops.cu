@@ -37,9 +37,11 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
 //   power of two; q = e4m3(n / s)
 // The statistics are those of the rounded h, which is what the next layer reads
 // back.  q is taken from the 32-bit n, not from y: one rounding fewer.
-// One CTA per row; a thread keeps its 8-column chunks in registers between the
-// sum of squares and the output, so every input is read once.  A block of 128
-// columns is 16 neighbouring lanes.
+// A CTA walks over rows; a thread keeps its 8-column chunks in registers between the
+// sum of squares and the output, so every input is read once, and has the next row's
+// inputs on their way meanwhile.  A block of 128 columns is 16 neighbouring lanes.
+// Bound by HBM: 16384 x 4096 with residual and both outputs, 604 MB, takes 102 us, 5.9 TB/s
+// (one CTA per row, without the loads ahead: 114 us).
 // ---------------------------------------------------------------------------
 struct NormArgs {
     const uint4 *x, *res;
@@ -49,6 +51,7 @@ struct NormArgs {
     void *s;
     float eps, inv_d;
     int chunks;  // D / 8
+    long long T;
     int weight_bf16, ue8m0, s_f32;
 };
 
@@ -58,105 +61,125 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+// CTAs of 256 threads that an SM holds at once, by chunks per thread (registers).
+constexpr int norm_ctas(int ch) { return ch <= 1 ? 6 : ch <= 2 ? 4 : ch <= 4 ? 2 : 1; }
+
 template <int CH>
-__global__ void __launch_bounds__(256) k_rms_norm_quant(const __grid_constant__ NormArgs p) {
-    __shared__ float part[8];
+__global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __grid_constant__ NormArgs p) {
+    __shared__ float parts[2][8];
     const int nt = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const size_t row = (size_t)blockIdx.x * p.chunks;
-    float v[CH][8];
-    float ss = 0.f;
+    uint4 nx[CH], nr[CH];
+    auto load = [&](long long t) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const int c = threadIdx.x + i * nt;
-        if (c < p.chunks) {
-            const uint4 a = __ldg(p.x + row + c);
-            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = bf2(u[j]);
-                v[i][2 * j] = f.x;
-                v[i][2 * j + 1] = f.y;
+        for (int i = 0; i < CH; ++i) {
+            const int c = threadIdx.x + i * nt;
+            if (c < p.chunks) {
+                nx[i] = __ldg(p.x + t * p.chunks + c);
+                if (p.res) nr[i] = __ldg(p.res + t * p.chunks + c);
             }
-            if (p.res) {
-                const uint4 b = __ldg(p.res + row + c);
-                const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-                uint32_t o[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = bf2(w[j]);
-                    o[j] = pack_bf2(v[i][2 * j] + f.x, v[i][2 * j + 1] + f.y);
-                    const float2 r = bf2(o[j]);
-                    v[i][2 * j] = r.x;
-                    v[i][2 * j + 1] = r.y;
-                }
-                p.h[row + c] = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
         }
-    }
+    };
+    pdl_launch_dependents();
+    pdl_wait();
+    if (blockIdx.x < p.T) load(blockIdx.x);
+    int flip = 0;
+    for (long long t = blockIdx.x; t < p.T; t += gridDim.x, flip ^= 1) {
+        const size_t row = (size_t)t * p.chunks;
+        float *part = parts[flip];
+        float v[CH][8];
+        float ss = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (lane == 0) part[warp] = ss;
-    __syncthreads();
-    ss = 0.f;
-    for (int w = 0; w < nt / 32; ++w) ss += part[w];
-    const float rstd = rsqrtf(ss * p.inv_d + p.eps);
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const int c = threadIdx.x + i * nt;
-        const bool on = c < p.chunks;  // whole groups of 16 lanes: chunks is a multiple of 16
-        float amax = 0.f;
-        if (on) {
-            float w[8];
-            if (p.weight_bf16) {
-                const uint4 a = __ldg((const uint4 *)p.weight + c);
-                const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+        for (int i = 0; i < CH; ++i) {
+            const int c = threadIdx.x + i * nt;
+            if (c < p.chunks) {
+                const uint32_t u[4] = {nx[i].x, nx[i].y, nx[i].z, nx[i].w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float2 f = bf2(u[j]);
-                    w[2 * j] = f.x;
-                    w[2 * j + 1] = f.y;
+                    v[i][2 * j] = f.x;
+                    v[i][2 * j + 1] = f.y;
                 }
+                if (p.res) {
+                    const uint32_t w[4] = {nr[i].x, nr[i].y, nr[i].z, nr[i].w};
+                    uint32_t o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = bf2(w[j]);
+                        o[j] = pack_bf2(v[i][2 * j] + f.x, v[i][2 * j + 1] + f.y);
+                        const float2 r = bf2(o[j]);
+                        v[i][2 * j] = r.x;
+                        v[i][2 * j + 1] = r.y;
+                    }
+                    p.h[row + c] = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+            }
+        }
+        if (t + gridDim.x < p.T) load(t + gridDim.x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (lane == 0) part[warp] = ss;
+        __syncthreads();
+        ss = 0.f;
+        for (int w = 0; w < nt / 32; ++w) ss += part[w];
+        const float rstd = rsqrtf(ss * p.inv_d + p.eps);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int c = threadIdx.x + i * nt;
+            const bool on = c < p.chunks;  // whole groups of 16 lanes: chunks is a multiple of 16
+            float amax = 0.f;
+            if (on) {
+                float w[8];
+                if (p.weight_bf16) {
+                    const uint4 a = __ldg((const uint4 *)p.weight + c);
+                    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = bf2(u[j]);
+                        w[2 * j] = f.x;
+                        w[2 * j + 1] = f.y;
+                    }
+                } else {
+                    const float4 a = __ldg((const float4 *)p.weight + 2 * c), b = __ldg((const float4 *)p.weight + 2 * c + 1);
+                    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+                    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[i][j] = v[i][j] * rstd * w[j];
+                    amax = max_nan(amax, fabsf(v[i][j]));
+                }
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            if (!on) continue;
+            // NaN passes through the maximum, so it reaches the scale as it does in n
+            float s = max_nan(amax, 1e-4f) * (1.0f / 448.0f);
+            uint32_t byte = 0;
+            if (p.ue8m0) {
+                const uint32_t b = __float_as_uint(s);
+                byte = s < CUDART_INF_F ? (b + 0x7fffffu) >> 23 : 0xffu;
+                s = byte < 0xffu ? __uint_as_float(byte << 23) : CUDART_NAN_F;
+            }
+            uint32_t lo, hi;
+            if (p.ue8m0) {
+                const float inv = 1.0f / s;  // exact
+                lo = f32x2_to_e4m3x2(v[i][0] * inv, v[i][1] * inv) | (uint32_t)f32x2_to_e4m3x2(v[i][2] * inv, v[i][3] * inv) << 16;
+                hi = f32x2_to_e4m3x2(v[i][4] * inv, v[i][5] * inv) | (uint32_t)f32x2_to_e4m3x2(v[i][6] * inv, v[i][7] * inv) << 16;
             } else {
-                const float4 a = __ldg((const float4 *)p.weight + 2 * c), b = __ldg((const float4 *)p.weight + 2 * c + 1);
-                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-                w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+                lo = f32x2_to_e4m3x2(v[i][0] / s, v[i][1] / s) | (uint32_t)f32x2_to_e4m3x2(v[i][2] / s, v[i][3] / s) << 16;
+                hi = f32x2_to_e4m3x2(v[i][4] / s, v[i][5] / s) | (uint32_t)f32x2_to_e4m3x2(v[i][6] / s, v[i][7] / s) << 16;
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[i][j] = v[i][j] * rstd * w[j];
-                amax = max_nan(amax, fabsf(v[i][j]));
+            p.q[row + c] = make_uint2(lo, hi);
+            if (p.y)
+                p.y[row + c] = make_uint4(pack_bf2(v[i][0], v[i][1]), pack_bf2(v[i][2], v[i][3]),
+                                          pack_bf2(v[i][4], v[i][5]), pack_bf2(v[i][6], v[i][7]));
+            if ((lane & 15) == 0) {
+                const size_t at = (row + c) >> 4;
+                if (p.s_f32) ((float *)p.s)[at] = s;
+                else ((uint8_t *)p.s)[at] = (uint8_t)byte;
             }
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (!on) continue;
-        // NaN passes through the maximum, so it reaches the scale as it does in n
-        float s = max_nan(amax, 1e-4f) * (1.0f / 448.0f);
-        uint32_t byte = 0;
-        if (p.ue8m0) {
-            const uint32_t b = __float_as_uint(s);
-            byte = s < CUDART_INF_F ? (b + 0x7fffffu) >> 23 : 0xffu;
-            s = byte < 0xffu ? __uint_as_float(byte << 23) : CUDART_NAN_F;
-        }
-        uint32_t lo, hi;
-        if (p.ue8m0) {
-            const float inv = 1.0f / s;  // exact
-            lo = f32x2_to_e4m3x2(v[i][0] * inv, v[i][1] * inv) | (uint32_t)f32x2_to_e4m3x2(v[i][2] * inv, v[i][3] * inv) << 16;
-            hi = f32x2_to_e4m3x2(v[i][4] * inv, v[i][5] * inv) | (uint32_t)f32x2_to_e4m3x2(v[i][6] * inv, v[i][7] * inv) << 16;
-        } else {
-            lo = f32x2_to_e4m3x2(v[i][0] / s, v[i][1] / s) | (uint32_t)f32x2_to_e4m3x2(v[i][2] / s, v[i][3] / s) << 16;
-            hi = f32x2_to_e4m3x2(v[i][4] / s, v[i][5] / s) | (uint32_t)f32x2_to_e4m3x2(v[i][6] / s, v[i][7] / s) << 16;
-        }
-        p.q[row + c] = make_uint2(lo, hi);
-        if (p.y)
-            p.y[row + c] = make_uint4(pack_bf2(v[i][0], v[i][1]), pack_bf2(v[i][2], v[i][3]),
-                                      pack_bf2(v[i][4], v[i][5]), pack_bf2(v[i][6], v[i][7]));
-        if ((lane & 15) == 0) {
-            const size_t at = (row + c) >> 4;
-            if (p.s_f32) ((float *)p.s)[at] = s;
-            else ((uint8_t *)p.s)[at] = (uint8_t)byte;
         }
     }
 }
@@ -498,6 +521,8 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, N <= 8 ? 8 : 4) k_route_topk
     __shared__ uint32_t sm[ROUTE_WARPS][32 * N];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long t = (long long)blockIdx.x * ROUTE_WARPS + warp;
+    pdl_launch_dependents();
+    pdl_wait();
     if (t >= p.T) return;
     float z[N], bias[N];
 #pragma unroll
@@ -568,7 +593,8 @@ __device__ __forceinline__ void disp_load(const DispArgs &p, int i0, int hi, int
 
 __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_count(const __grid_constant__ DispArgs p) {
     __shared__ int cnt[DISP_MAX_E];
-    pdl_launch_dependents();
+    pdl_wait();
+    pdl_launch_dependents();  // (after the wait: the placing kernel reads the indices without one)
     const int warp = threadIdx.x >> 5;
     const int lo = min(p.pairs, (blockIdx.x * DISP_WARPS + warp) * p.run), hi = min(p.pairs, lo + p.run);
     int e[DISP_LANE];
@@ -593,6 +619,8 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid
     const int lo = min(p.pairs, (blockIdx.x * DISP_WARPS + warp) * p.run), hi = min(p.pairs, lo + p.run);
     const bool whole = hi - lo <= DISP_STEP;  // the run stays in registers
     int e[DISP_LANE], ahead[DISP_LANE];
+    pdl_launch_dependents();
+    if (p.nchunks == 1) pdl_wait();
     disp_load(p, lo, hi, e);
     for (int x = lane; x < p.E; x += 32) cnt[warp][x] = 0;
     for (int x = threadIdx.x; x < p.E; x += blockDim.x) total[x] = before[x] = 0;
@@ -689,6 +717,8 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid
 // in ascending row order (ascending expert, the layer's own order), in 32 bits.
 // A slot outside [0, R) adds nothing.  One CTA per token and 2048 columns, 8
 // columns per thread; the token's slots are sorted once per CTA.
+// Bound by HBM: 8192 tokens x 8 rows of 4096 with the shared rows, 671 MB, take 108 us,
+// 6.2 TB/s (one row's load at a time: 117 us).
 // ---------------------------------------------------------------------------
 constexpr int COMB_MAX_K = 16;
 
@@ -705,6 +735,8 @@ __global__ void __launch_bounds__(256) k_combine(const __grid_constant__ CombArg
     __shared__ float weight[COMB_MAX_K];
     const size_t t = blockIdx.x;
     const int lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    pdl_wait();
     if (threadIdx.x < 32) {
         const int s = lane < p.k ? p.slots[t * p.k + lane] : -1;
         const float w = lane < p.k && p.weights ? p.weights[t * p.k + lane] : 1.0f;
@@ -724,17 +756,25 @@ __global__ void __launch_bounds__(256) k_combine(const __grid_constant__ CombArg
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int i = 0; i < p.k; ++i) {
-        const int s = slot[i];
-        if (s < 0 || s >= p.R) continue;
-        const uint4 a = __ldg(p.rows + (size_t)s * p.chunks + c);
-        const float w = weight[i];
-        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+    for (int i0 = 0; i0 < p.k; i0 += 8) {  // eight rows' loads in flight
+        uint4 a[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = bf2(u[j]);
-            acc[2 * j] += w * f.x;
-            acc[2 * j + 1] += w * f.y;
+        for (int i = 0; i < 8; ++i) {
+            const int s = i0 + i < p.k ? slot[i0 + i] : -1;
+            if (s >= 0 && s < p.R) a[i] = __ldg(p.rows + (size_t)s * p.chunks + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int s = i0 + i < p.k ? slot[i0 + i] : -1;
+            if (s < 0 || s >= p.R) continue;
+            const float w = weight[i0 + i];
+            const uint32_t u[4] = {a[i].x, a[i].y, a[i].z, a[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = bf2(u[j]);
+                acc[2 * j] += w * f.x;
+                acc[2 * j + 1] += w * f.y;
+            }
         }
     }
     const size_t at = t * p.chunks + c;
@@ -758,10 +798,7 @@ __global__ void __launch_bounds__(256) k_combine(const __grid_constant__ CombArg
     }
 }
 
-int launched(const char *what) {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? WF_OK : cuda_fail(e, what);
-}
+int launched(cudaError_t e, const char *what) { return e == cudaSuccess ? WF_OK : cuda_fail(e, what); }
 
 bool misaligned(const void *p, uintptr_t to) { return (uintptr_t)p % to != 0; }
 
@@ -787,20 +824,18 @@ int wf_rms_norm_quant(const void *x, const void *residual, const void *weight, i
     NormArgs p;
     p.x = (const uint4 *)x; p.res = (const uint4 *)residual; p.weight = weight;
     p.y = (uint4 *)y; p.h = (uint4 *)h; p.q = (uint2 *)q; p.s = s;
-    p.eps = eps; p.inv_d = 1.0f / (float)D; p.chunks = (int)(D / 8);
+    p.eps = eps; p.inv_d = 1.0f / (float)D; p.chunks = (int)(D / 8); p.T = T;
     p.weight_bf16 = weight_bf16 != 0; p.ue8m0 = ue8m0 != 0; p.s_f32 = scale_kind == WF_SCALE_F32;
     const int ch = (p.chunks + 255) / 256;
     const int nt = ch > 1 ? 256 : (p.chunks + 31) / 32 * 32;
-    const unsigned g = (unsigned)T;
-    cudaStream_t st = (cudaStream_t)stream;
-    switch (ch) {
-        case 1: k_rms_norm_quant<1><<<g, nt, 0, st>>>(p); break;
-        case 2: k_rms_norm_quant<2><<<g, nt, 0, st>>>(p); break;
-        case 3: case 4: k_rms_norm_quant<4><<<g, nt, 0, st>>>(p); break;
-        default: k_rms_norm_quant<8><<<g, nt, 0, st>>>(p); break;
-    }
-    wf::host::counted();
-    return launched("rms_norm_quant launch");
+    const int sms = wf::host::sm_count();
+    if (sms <= 0) return fail(WF_E_CUDA, "no CUDA device");
+    const int ct = ch <= 2 ? ch : ch <= 4 ? 4 : 8;
+    const int per_sm = ct > 1 ? norm_ctas(ct) : norm_ctas(1) * 256 / nt < 32 ? norm_ctas(1) * 256 / nt : 32;
+    const int64_t most = (int64_t)sms * per_sm;
+    const dim3 g((unsigned)(T < most ? T : most));
+    auto k = ct == 1 ? k_rms_norm_quant<1> : ct == 2 ? k_rms_norm_quant<2> : ct == 4 ? k_rms_norm_quant<4> : k_rms_norm_quant<8>;
+    return launched(wf::host::launch_pdl(k, g, nt, 0, (cudaStream_t)stream, p), "rms_norm_quant launch");
 }
 
 int wf_route_topk(const void *logits, int32_t logits_bf16, const float *bias, int64_t T, int32_t E, int32_t topk,
@@ -828,15 +863,10 @@ int wf_route_topk(const void *logits, int32_t logits_bf16, const float *bias, in
     p.magic = ((1u << 20) + p.per - 1) / p.per;
     p.part = 0;
     while (2 << p.part <= 32 / n_groups) ++p.part;
-    const unsigned g = (unsigned)((T + ROUTE_WARPS - 1) / ROUTE_WARPS);
-    cudaStream_t st = (cudaStream_t)stream;
+    const dim3 g((unsigned)((T + ROUTE_WARPS - 1) / ROUTE_WARPS));
     const int per = (E + 31) / 32;
-    if (per <= 2) k_route_topk<2><<<g, 32 * ROUTE_WARPS, 0, st>>>(p);
-    else if (per <= 4) k_route_topk<4><<<g, 32 * ROUTE_WARPS, 0, st>>>(p);
-    else if (per <= 8) k_route_topk<8><<<g, 32 * ROUTE_WARPS, 0, st>>>(p);
-    else k_route_topk<16><<<g, 32 * ROUTE_WARPS, 0, st>>>(p);
-    wf::host::counted();
-    return launched("route_topk launch");
+    auto k = per <= 2 ? k_route_topk<2> : per <= 4 ? k_route_topk<4> : per <= 8 ? k_route_topk<8> : k_route_topk<16>;
+    return launched(wf::host::launch_pdl(k, g, 32 * ROUTE_WARPS, 0, (cudaStream_t)stream, p), "route_topk launch");
 }
 
 // Chunks of `pairs` pairs, and the pairs of a warp's run: short runs for few pairs, so that the
@@ -884,24 +914,10 @@ int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32
     p.base = (int)expert_offset; p.hist = (int *)workspace; p.offsets = offsets; p.tokens = tokens; p.slots = slots;
     p.nchunks = disp_chunks(p.pairs, &p.run);
     cudaStream_t st = (cudaStream_t)stream;
-    if (p.nchunks == 1) {
-        k_dispatch_place<<<1, 32 * DISP_WARPS, 0, st>>>(p);
-        wf::host::counted();
-        return launched("expert_dispatch launch");
-    }
-    k_dispatch_count<<<p.nchunks, 32 * DISP_WARPS, 0, st>>>(p);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.nchunks);
-    cfg.blockDim = dim3(32 * DISP_WARPS);
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_dispatch_place, p);
-    wf::host::counted(2);
-    return e == cudaSuccess ? launched("expert_dispatch launch") : cuda_fail(e, "expert_dispatch launch");
+    cudaError_t e = cudaSuccess;
+    if (p.nchunks > 1) e = wf::host::launch_pdl(k_dispatch_count, dim3(p.nchunks), 32 * DISP_WARPS, 0, st, p);
+    if (e == cudaSuccess) e = wf::host::launch_pdl(k_dispatch_place, dim3(p.nchunks), 32 * DISP_WARPS, 0, st, p);
+    return launched(e, "expert_dispatch launch");
 }
 
 int wf_expert_combine(const void *rows, int64_t R, const int32_t *slots, const float *weights, const void *shared,
@@ -919,9 +935,7 @@ int wf_expert_combine(const void *rows, int64_t R, const int32_t *slots, const f
     p.R = (int)R; p.k = topk; p.chunks = (int)(D / 8); p.y_f32 = y_f32 != 0;
     const int nt = p.chunks >= 256 ? 256 : (p.chunks + 31) / 32 * 32;
     const dim3 g((unsigned)T, (unsigned)((p.chunks + nt - 1) / nt));
-    k_combine<<<g, nt, 0, (cudaStream_t)stream>>>(p);
-    wf::host::counted();
-    return launched("expert_combine launch");
+    return launched(wf::host::launch_pdl(k_combine, g, nt, 0, (cudaStream_t)stream, p), "expert_combine launch");
 }
 
 }  // extern "C"
