@@ -345,8 +345,8 @@ int wf_route_topk(const void *logits, int32_t logits_bf16, const float *bias, in
  * outside them (-1 among them) gets no row.  offsets [n_experts + 1]: expert e
  * owns rows [offsets[e], offsets[e+1]); tokens [T * topk]: the token of each
  * row, -1 behind the last; slots [T, topk]: the row of each pair, or -1.  Rows
- * are in order of (expert, token, slot).  The workspace (0 bytes for few pairs: then
- * it may be NULL) needs no initial value. */
+ * are in order of (expert, token, slot).  The workspace (16-byte aligned; 0 bytes
+ * for few pairs: then it may be NULL) needs no initial value. */
 size_t wf_expert_dispatch_workspace_bytes(int64_t T, int32_t topk, int32_t n_experts);
 int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32_t topk,
                        int32_t n_experts, int64_t expert_offset, int32_t *offsets, int32_t *tokens,

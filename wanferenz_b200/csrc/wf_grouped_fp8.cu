@@ -15,6 +15,10 @@
 // byte per 128 K repeated for its four 32-wide products) and sums the whole of K in
 // TMEM.  Otherwise each 128-wide K step's product goes to a fresh accumulator, and the
 // worker warps scale and add it in 32-bit registers while the next step multiplies.
+// For many rows per expert those sums are all that counts, and the sides change places
+// (k_grouped_f32_wide): a token per TMEM lane, so that a thread's scale is one register.
+// (A scale per column comes from shared memory, 4 bytes a lane and column whether the
+// lanes read the same ones or not: 131 KB a K step, as many cycles as the whole product.)
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -38,17 +42,16 @@ constexpr int SGRP = 8;                 // K steps per group of scales
 constexpr int FEW = 64;                 // rows per expert up to which tiles are narrow and row lists gathered in place
 constexpr int W_PROD = 0, W_MMA = 1, WORKERS = 8;
 constexpr int SMEM_MAX = 232448;
+constexpr int TAB_BYTES = (3 * MAX_E + 4) * 4;  // per expert: first row, rows, first token tile
 
-// One kernel per way of applying scales and per tile width.  NT: tokens per tile, at most.  Narrow
-// tiles, for few rows per expert, leave room for ten stages and for accumulators ahead of the
-// workers: there the weights' stream from HBM is all that counts, and nothing may pause it.
+// NT: tokens per tile, at most.  Narrow tiles, for few rows per expert, leave room for ten stages and
+// for accumulators ahead of the workers: there the weights' stream from HBM is all that counts, and
+// nothing may pause it.
 template <bool E8, int NT>
 struct Plan {
-    // e8m0: 4 scale warps (one per TMEM lane quadrant); f32: 2, and the wide tile's accumulators need
-    // the registers of a smaller block
+    // e8m0: 4 scale warps, one per TMEM lane quadrant; f32: 2
     static constexpr int SCALE0 = E8 ? 4 : 2, SCALERS = E8 ? 4 : 2, WORK0 = SCALE0 + SCALERS;
     static constexpr int THREADS = 32 * (WORK0 + WORKERS);
-    static constexpr bool SPLIT = !E8 && NT == 256;      // workers take registers from the other roles
     static constexpr int ABYTES = 128 * 128, BBYTES = NT / 2 * 128, STAGE = ABYTES + BBYTES;
     static constexpr int STAGES = NT == 256 ? 6 : 10;
     // TMEM: sums of whole tiles (e8m0) and two groups of scale factors, or products of K steps (f32)
@@ -57,13 +60,11 @@ struct Plan {
     static constexpr uint32_t COL_SFA = 256, COL_SFB = COL_SFA + 2 * SGRP * 4;
     static constexpr int NBAR = 2 * STAGES + 2 * NACC + 5;
     static constexpr int OFF_S = STAGES * STAGE;         // scales: [2][SGRP][NT] f32 or [2][NT] x 8 bytes
-    static constexpr int OFF_LO = OFF_S + 2 * SGRP * NT * 4;  // [MAX_E] first row
-    static constexpr int OFF_CNT = OFF_LO + MAX_E * 4;   // [MAX_E] rows
-    static constexpr int OFF_T = OFF_CNT + MAX_E * 4;    // [MAX_E + 1] first token tile
-    static constexpr int OFF_BAR = OFF_T + (MAX_E + 4) * 4;
+    static constexpr int OFF_TAB = OFF_S + 2 * SGRP * NT * 4;
+    static constexpr int OFF_BAR = OFF_TAB + TAB_BYTES;
     static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
     static_assert(SMEM <= SMEM_MAX && OFF_BAR % 8 == 0, "shared memory");
-    static_assert(!E8 || (NACC * NT <= 256 && COL_SFB + 2 * SGRP * SFB <= 512), "tensor memory");
+    static_assert(E8 ? NACC * NT <= 256 && COL_SFB + 2 * SGRP * SFB <= 512 : NT == 64, "tensor memory");
 };
 
 struct Args {
@@ -228,21 +229,59 @@ struct Tile {
     int e, n0, r0, nrow, width;
 };
 
-// Tiles of this CTA pair in order; within an expert the weight tile runs fastest.
+// Every expert's rows, clamped to the R rows there are, and its first token tile, in shared memory.
+struct Table {
+    int *lo, *cnt, *first;
+    __device__ explicit Table(uint8_t *at)
+        : lo(reinterpret_cast<int *>(at)), cnt(lo + MAX_E), first(cnt + MAX_E) {}
+    // By all threads; complete for the caller's next barrier.
+    __device__ void fill(const Args &p, int nt) const {
+        for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+            const int a = min(max(p.offsets[e], 0), p.R), b = min(max(p.offsets[e + 1], 0), p.R);
+            lo[e] = a;
+            cnt[e] = max(b - a, 0);
+        }
+        __syncthreads();
+        if (threadIdx.x >= 32) return;
+        const int lane = threadIdx.x;
+        int sum = 0, own[MAX_E / 32];
+#pragma unroll
+        for (int j = 0; j < MAX_E / 32; ++j) {
+            const int e = lane * (MAX_E / 32) + j;
+            own[j] = sum;
+            if (e < p.E) sum += (cnt[e] + nt - 1) / nt;
+        }
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+#pragma unroll
+        for (int j = 0; j < MAX_E / 32; ++j) {
+            const int e = lane * (MAX_E / 32) + j;
+            if (e < p.E) first[e] = incl - sum + own[j];
+        }
+        if (lane == 31) first[p.E] = incl;
+    }
+};
+
+// Tiles of a CTA (pair) in order; within an expert the tile of 256 weight rows runs fastest.
 struct Walk {
-    const int *lo, *cnt, *first;
+    Table tab;
     int E, nn, step, e;
     long long i;
-    __device__ bool next(Tile &t) {
-        while (e < E && i >= (long long)first[e + 1] * nn) ++e;
+    // Cuts an expert's rows into tiles of equal width (even: a multiple of 32) or of `fixed` rows.
+    __device__ bool next(Tile &t, int fixed = 0) {
+        while (e < E && i >= (long long)tab.first[e + 1] * nn) ++e;
         if (e >= E) return false;
-        const int local = (int)(i - (long long)first[e] * nn);
-        const int nt = first[e + 1] - first[e], c = cnt[e];
+        const int local = (int)(i - (long long)tab.first[e] * nn);
+        const int nt = tab.first[e + 1] - tab.first[e], c = tab.cnt[e];
         t.e = e;
         t.n0 = local % nn * 256;
-        t.width = ((c + nt - 1) / nt + 31) / 32 * 32;  // cta_group::2 takes N in steps of 32
+        t.width = fixed ? fixed : ((c + nt - 1) / nt + 31) / 32 * 32;  // cta_group::2 takes N in steps of 32
         const int j = local / nn * t.width;
-        t.r0 = lo[e] + j;
+        t.r0 = tab.lo[e] + j;
         t.nrow = min(t.width, c - j);
         i += step;
         return true;
@@ -282,8 +321,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
     uint64_t *sf_full = acc_free + NACC, *sf_empty = sf_full + 2, *fin = sf_empty + 2;
     uint32_t *tmem_base = reinterpret_cast<uint32_t *>(bar + L::NBAR);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_base + 1);
-    int *lo = reinterpret_cast<int *>(base + L::OFF_LO), *cnt = reinterpret_cast<int *>(base + L::OFF_CNT);
-    int *first = reinterpret_cast<int *>(base + L::OFF_T);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int nks = p.K / 128, nn = (p.N + 255) / 256, nb = (p.N + 127) / 128;
@@ -305,44 +342,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
     if (warp == W_MMA) tmem_alloc2(tmem_base, 512);
     pdl_launch_dependents();
     pdl_wait();
-    // every expert's rows, clamped to the R rows there are, and its first token tile
-    for (int e = threadIdx.x; e < p.E; e += L::THREADS) {
-        const int a = min(max(p.offsets[e], 0), p.R), b = min(max(p.offsets[e + 1], 0), p.R);
-        lo[e] = a;
-        cnt[e] = max(b - a, 0);
-    }
-    __syncthreads();
-    if (warp == W_PROD) {
-        int sum = 0, own[MAX_E / 32];
-#pragma unroll
-        for (int j = 0; j < MAX_E / 32; ++j) {
-            const int e = lane * (MAX_E / 32) + j;
-            own[j] = sum;
-            if (e < p.E) sum += (cnt[e] + NT - 1) / NT;
-        }
-        int incl = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-        }
-#pragma unroll
-        for (int j = 0; j < MAX_E / 32; ++j) {
-            const int e = lane * (MAX_E / 32) + j;
-            if (e < p.E) first[e] = incl - sum + own[j];
-        }
-        if (lane == 31) first[p.E] = incl;
-    }
+    const Table tab(base + L::OFF_TAB);
+    tab.fill(p, NT);
     fence_before_sync();
     __syncthreads();
     cluster_sync();
     fence_after_sync();
     const uint32_t tm = *tmem_base;
-    Walk walk{lo, cnt, first, p.E, nn, (int)(gridDim.x / 2), 0, (long long)(blockIdx.x / 2)};
+    Walk walk{tab, p.E, nn, (int)(gridDim.x / 2), 0, (long long)(blockIdx.x / 2)};
     Tile t;
 
     if (warp == W_PROD) {
-        if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         int gs = 0;
         bool ok = true;
         // Narrow tiles read most weights once, wide ones several times: evict-first took 1536 rows
@@ -394,7 +404,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
             while (clock64() - t0 < 8000000) {}
         }
     } else if (warp == W_MMA) {
-        if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // The whole warp walks the loop and one elected lane issues, so that descriptors stay in
         // uniform registers (a loop run by one lane alone moves every operand there by itself:
         // 850 cycles per K step, more than its product takes).
@@ -513,8 +522,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
             for (int u = max(0, sg - 2); ok && u < sg; ++u) ok = twait(sf_empty + (u & 1), (u / 2) & 1, abort, p.limit);
         } else {
             // token scale x weight scale of each K step into shared memory
-            if constexpr (L::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-            float *sa = reinterpret_cast<float *>(base + L::OFF_S);
+                float *sa = reinterpret_cast<float *>(base + L::OFF_S);
             const int i = threadIdx.x - 32 * L::SCALE0;  // this thread: tokens i, i + 64, ...
             int sg = 0;
             bool ok = true;
@@ -552,7 +560,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
     } else {
         // workers: warp (q, half) takes the 32 weight rows of TMEM lane quadrant q and half of the
         // widest tile's tokens
-        if constexpr (L::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int q = warp & 3, half = (warp - L::WORK0) >> 2;
         const uint32_t col = tm + ((uint32_t)(32 * q) << 16) + HALF * half;
         const float *sa = reinterpret_cast<const float *>(base + L::OFF_S) + HALF * half;
@@ -651,6 +658,208 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
     }
 }
 
+// ---------------------------------------------------------------------------
+// f32 scales, many rows per expert: 128 tokens x 256 weight rows a tile, one CTA each
+// ---------------------------------------------------------------------------
+namespace wide {
+constexpr int MT = 128, NW = 256, STAGES = 4, ABYTES = MT * 128, STAGE = ABYTES + NW * 128;
+constexpr int W_WORK0 = 4, THREADS = 32 * (W_WORK0 + WORKERS);
+constexpr int NBAR = 2 * STAGES + 5;
+constexpr int OFF_TAB = STAGES * STAGE, OFF_BAR = OFF_TAB + TAB_BYTES, SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
+static_assert(SMEM <= SMEM_MAX && OFF_BAR % 8 == 0, "shared memory");
+// Registers: a worker holds 128 sums and 64 loaded products; the split of what the block was
+// launched with (REGS a thread, checked before the first launch) must not ask for more.
+constexpr int REGS = 168;
+static_assert(256 * 216 + 128 * 72 <= THREADS * REGS, "register split");
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+    // f32 += e4m3 x e4m3, M = 128, N = 256, both operands K-major
+    constexpr uint32_t idesc = 1u << 4 | (NW >> 3) << 17 | (MT >> 4) << 24;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&v)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+        "%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,"
+        "%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]),
+          "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]),
+          "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]),
+          "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]),
+          "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+        : "r"(taddr)
+        : "memory");
+}
+// (d0, d1) += s * (a, b), two 32-bit operations in one instruction
+__device__ __forceinline__ void fma2(float &d0, float &d1, float s, uint32_t a, uint32_t b) {
+    asm("{\n\t.reg .b64 d, s, v;\n\t"
+        "mov.b64 d, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 v, {%3, %4};\n\t"
+        "fma.rn.f32x2 d, s, v, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(d0), "+f"(d1)
+        : "f"(s), "r"(a), "r"(b));
+}
+}  // namespace wide
+
+__global__ void __launch_bounds__(wide::THREADS, 1) k_grouped_f32_wide(const __grid_constant__ Args p) {
+    using namespace wide;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bar = reinterpret_cast<uint64_t *>(base + OFF_BAR);
+    uint64_t *full = bar, *empty = bar + STAGES, *acc_ready = empty + STAGES, *acc_free = acc_ready + 2, *fin = acc_free + 2;
+    uint32_t *tmem_base = reinterpret_cast<uint32_t *>(bar + NBAR);
+    volatile int *abort = reinterpret_cast<volatile int *>(tmem_base + 1);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int nks = p.K / 128, nn = (p.N + NW - 1) / NW, nb = (p.N + 127) / 128;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+        for (int j = 0; j < 2; ++j) { mbar_init(acc_ready + j, 1); mbar_init(acc_free + j, WORKERS); }
+        mbar_init(fin, 1);
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == W_MMA) { tmem_alloc(tmem_base, 512); tmem_relinquish(); }
+    pdl_launch_dependents();
+    pdl_wait();
+    const Table tab(base + OFF_TAB);
+    tab.fill(p, MT);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tm = *tmem_base;
+    Walk walk{tab, p.E, nn, (int)gridDim.x, 0, (long long)blockIdx.x};
+    Tile t;
+
+    if (warp < W_WORK0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == W_PROD) {
+            int gs = 0;
+            bool ok = true;
+            while (ok && walk.next(t, MT)) {
+                const int mine = (t.nrow + 15) & ~15;  // rows loaded; lanes behind the last row are not stored
+                for (int ks = 0; ks < nks; ++ks, ++gs) {
+                    const int st = gs % STAGES;
+                    if (gs >= STAGES) ok = twait(empty + st, (gs / STAGES - 1) & 1, abort, p.limit);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    uint8_t *dst = base + st * STAGE;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(full + st, NW * 128 + mine * 128);
+                        tma_load_2d(dst + ABYTES, &p.tmW, ks * 128, t.e * p.N + t.n0, full + st);
+                        tma_load_2d(dst + ABYTES + 128 * 128, &p.tmW, ks * 128, t.e * p.N + t.n0 + 128, full + st);
+                    }
+                    __syncwarp();
+                    if (lane < 4 && mine & 128 >> lane) {
+                        const int at = mine & ~(0xff >> lane);
+                        tma_load_2d(dst + at * 128, &p.tmA[lane], ks * 128, t.r0 + at, full + st);
+                    }
+                }
+            }
+            if (*abort)  // the copies issued must land before the CTA's memory goes
+                for (int u = max(0, gs - STAGES); u < gs; ++u) wf_wait(full + u % STAGES, (u / STAGES) & 1, &g_err);
+        } else if (warp == W_MMA) {
+            const bool leader = elect_one();
+            const uint64_t ad0 = smem_desc_sw128(base), bd0 = smem_desc_sw128(base + ABYTES);
+            int st = 0, acc = 0;
+            uint32_t phase = 0, aphase = 1;
+            bool ok = true;
+            while (ok && walk.next(t, MT)) {
+                for (int ks = 0; ks < nks; ++ks) {
+                    ok = twait(acc_free + acc, aphase, abort, p.limit) && twait(full + st, phase, abort, p.limit);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    fence_after_sync();
+                    if (leader) {
+                        const uint64_t ad = ad0 + st * (STAGE / 16), bd = bd0 + st * (STAGE / 16);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma(tm + NW * acc, ad + 2 * j, bd + 2 * j, j != 0);
+                        commit(empty + st);
+                        commit(acc_ready + acc);
+                    }
+                    __syncwarp();
+                    if (++st == STAGES) { st = 0; phase ^= 1; }
+                    acc ^= 1;
+                    if (!acc) aphase ^= 1;
+                }
+            }
+            if (leader) commit(fin);  // TMEM goes only when every MMA is done
+            twait(fin, 0, abort, kWaitLimitCycles);
+        }
+    } else {
+        // worker (q, half): the 32 tokens of TMEM lane quadrant q, 128 weight rows (one block of scales)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int q = warp & 3, half = (warp - W_WORK0) >> 2;
+        const uint32_t col = tm + ((uint32_t)(32 * q) << 16) + 128 * half;
+        int acc = 0;
+        uint32_t aphase = 0;
+        bool ok = true;
+        while (ok && walk.next(t, MT)) {
+            const int row = 32 * q + lane;
+            bool valid;
+            const size_t ai = (size_t)source_row(p, t.r0 + min(row, t.nrow - 1), valid) * nks;
+            // the second block may lie past N: any scale does, nothing of it is stored
+            const size_t wi = ((size_t)t.e * nb + min(t.n0 / 128 + half, nb - 1)) * nks;
+            float sum[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) sum[j] = 0.f;
+            float next = scale_at(p.a_s, p.a_f32, ai) * scale_at(p.w_s, p.w_f32, wi);
+            for (int ks = 0; ks < nks; ++ks) {
+                const float s = next;
+                const int k1 = min(ks + 1, nks - 1);  // the next step's scale is on its way during this one
+                const float an = scale_at(p.a_s, p.a_f32, ai + k1), wn = scale_at(p.w_s, p.w_f32, wi + k1);
+                ok = twait(acc_ready + acc, aphase, abort, p.limit);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                fence_after_sync();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[64];
+                    tmem_ld64(col + NW * acc + 64 * c, v);
+                    tmem_wait_ld();
+                    if (c == 1) {
+                        fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_free + acc);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 64; j += 2) fma2(sum[64 * c + j], sum[64 * c + j + 1], s, v[j], v[j + 1]);
+                }
+                next = an * wn;
+                acc ^= 1;
+                if (!acc) aphase ^= 1;
+            }
+            if (!ok) break;
+            if (row < t.nrow) {
+                const int n0 = t.n0 + 128 * half;
+                uint4 *o = reinterpret_cast<uint4 *>(p.out + (size_t)(t.r0 + row) * p.N + n0);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    if (n0 + 8 * c >= p.N) break;
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(valid ? sum[8 * c + 2 * j] : 0.f, valid ? sum[8 * c + 2 * j + 1] : 0.f);
+                        y[j] = *reinterpret_cast<const uint32_t *>(&b);
+                    }
+                    o[c] = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == W_MMA) {
+        fence_after_sync();
+        tmem_dealloc(tm, 512);
+    }
+}
+
 // The listed rows of a in the product's order (rows that do not exist: row 0, their results are zeroed).
 constexpr int PACK_STEP = 4 * 256;
 __global__ void __launch_bounds__(256) k_pack_rows(const uint4 *a, const int *rows, const int *offsets, uint4 *out, int E,
@@ -693,9 +902,10 @@ int tensor_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t K, uint
     return WF_OK;
 }
 
-template <bool E8, int NT>
-cudaError_t launch(const Args &p, int sms, cudaStream_t st) {
-    using L = Plan<E8, NT>;
+// `kernel` with `ctas` CTAs for each of the units of work that fit the device, at most one per tile of
+// `nt` rows x 256 weight rows.
+template <void (*kernel)(const Args)>
+cudaError_t launch(const Args &p, int ctas, int nt, int threads, int smem, int sms, cudaStream_t st, int regs = 0) {
     // once per device (the attribute is the function's, whichever thread sets it)
     static std::atomic<uint64_t> ready{0};
     int dev = 0;
@@ -703,12 +913,21 @@ cudaError_t launch(const Args &p, int sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (dev > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(k_grouped_fp8<E8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
+        // a register split of more than the block is launched with would wait for ever
+        cudaFuncAttributes a;
+        e = cudaFuncGetAttributes(&a, kernel);
+        if (e != cudaSuccess) return e;
+        if (a.numRegs < regs) return cudaErrorInvalidConfiguration;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    const int64_t tiles = ((int64_t)p.R / NT + (p.E < p.R ? p.E : p.R)) * ((p.N + 255) / 256);
-    return host::launch_pdl(k_grouped_fp8<E8, NT>, dim3(2 * (unsigned)(tiles < sms / 2 ? tiles : sms / 2)), L::THREADS, L::SMEM, st, p);
+    const int64_t tiles = ((int64_t)p.R / nt + (p.E < p.R ? p.E : p.R)) * ((p.N + 255) / 256), most = sms / ctas;
+    return host::launch_pdl(kernel, dim3(ctas * (unsigned)(tiles < most ? tiles : most)), threads, smem, st, p);
+}
+template <bool E8, int NT>
+cudaError_t launch_pairs(const Args &p, int sms, cudaStream_t st) {
+    return launch<k_grouped_fp8<E8, NT>>(p, 2, NT, Plan<E8, NT>::THREADS, Plan<E8, NT>::SMEM, sms, st);
 }
 
 }  // namespace grp
@@ -772,8 +991,10 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
                                  (const uint4 *)a, rows, offsets, (uint4 *)workspace, (int)E, (int)M, (int)R, (int)(K / 16));
     }
     if (e == cudaSuccess)
-        e = e8 ? (few ? wf::grp::launch<true, 64>(p, sms, st) : wf::grp::launch<true, 256>(p, sms, st))
-               : (few ? wf::grp::launch<false, 64>(p, sms, st) : wf::grp::launch<false, 256>(p, sms, st));
+        e = few ? (e8 ? wf::grp::launch_pairs<true, 64>(p, sms, st) : wf::grp::launch_pairs<false, 64>(p, sms, st))
+            : e8 ? wf::grp::launch_pairs<true, 256>(p, sms, st)
+                 : wf::grp::launch<wf::grp::k_grouped_f32_wide>(p, 1, wf::grp::wide::MT, wf::grp::wide::THREADS,
+                                                                wf::grp::wide::SMEM, sms, st, wf::grp::wide::REGS);
     return e == cudaSuccess ? WF_OK : cuda_fail(e, "grouped_fp8_gemm launch");
 }
 

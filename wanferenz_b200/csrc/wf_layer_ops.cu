@@ -570,7 +570,8 @@ struct DispArgs {
     int idx64;
     int pairs, k, E, base;
     int run, nchunks;  // pairs per warp (a multiple of 32), chunks of DISP_WARPS runs
-    int *hist;         // [nchunks, E] when nchunks > 1
+    int row;           // E rounded up to a multiple of 4
+    int *hist;         // [nchunks, row] when nchunks > 1
     int *offsets, *tokens, *slots;
 };
 
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_count(const __grid
         if (i0 < hi) disp_load(p, i0, hi, e);
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < p.E; x += blockDim.x) p.hist[(size_t)blockIdx.x * p.E + x] = cnt[x];
+    for (int x = threadIdx.x; x < p.row; x += blockDim.x) p.hist[(size_t)blockIdx.x * p.row + x] = x < p.E ? cnt[x] : 0;
 }
 
 __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid_constant__ DispArgs p) {
@@ -642,16 +643,23 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid
     if (p.nchunks > 1) {
         __syncthreads();
         pdl_wait();
-        for (int x = lane; x < p.E; x += 32) {
-            int pre = 0, all = 0;
-#pragma unroll 4
-            for (int c = warp; c < p.nchunks; c += DISP_WARPS) {
-                const int n = __ldcg(p.hist + (size_t)c * p.E + x);
-                all += n;
-                if (c < (int)blockIdx.x) pre += n;
+        // four experts a thread, the chunks dealt out over the groups of threads that cover a row
+        const int quads = p.row / 4, g = threadIdx.x / quads, groups = blockDim.x / quads, x = threadIdx.x % quads * 4;
+        if (g < groups) {
+            int4 pre = make_int4(0, 0, 0, 0), all = pre;
+#pragma unroll 8
+            for (int c = g; c < p.nchunks; c += groups) {
+                const int4 n = __ldcg(reinterpret_cast<const int4 *>(p.hist + (size_t)c * p.row + x));
+                const int m = c < (int)blockIdx.x ? -1 : 0;
+                all.x += n.x; all.y += n.y; all.z += n.z; all.w += n.w;
+                pre.x += n.x & m; pre.y += n.y & m; pre.z += n.z & m; pre.w += n.w & m;
             }
-            if (all) atomicAdd(&total[x], all);
-            if (pre) atomicAdd(&before[x], pre);
+            const int va[4] = {all.x, all.y, all.z, all.w}, vp[4] = {pre.x, pre.y, pre.z, pre.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (va[j]) atomicAdd(&total[x + j], va[j]);
+                if (vp[j]) atomicAdd(&before[x + j], vp[j]);
+            }
         }
     }
     __syncthreads();
@@ -717,8 +725,8 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid
 // in ascending row order (ascending expert, the layer's own order), in 32 bits.
 // A slot outside [0, R) adds nothing.  One CTA per token and 2048 columns, 8
 // columns per thread; the token's slots are sorted once per CTA.
-// Bound by HBM: 8192 tokens x 8 rows of 4096 with the shared rows, 671 MB, take 108 us,
-// 6.2 TB/s (one row's load at a time: 117 us).
+// Bound by HBM: 8192 tokens x 8 rows of 4096 with the shared rows, 671 MB, take 104 us,
+// 6.4 TB/s (one row's load at a time: 117 us; eight, with fewer CTAs on an SM: 112 us).
 // ---------------------------------------------------------------------------
 constexpr int COMB_MAX_K = 16;
 
@@ -756,15 +764,15 @@ __global__ void __launch_bounds__(256) k_combine(const __grid_constant__ CombArg
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    for (int i0 = 0; i0 < p.k; i0 += 8) {  // eight rows' loads in flight
-        uint4 a[8];
+    for (int i0 = 0; i0 < p.k; i0 += 4) {  // four rows' loads in flight
+        uint4 a[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const int s = i0 + i < p.k ? slot[i0 + i] : -1;
             if (s >= 0 && s < p.R) a[i] = __ldg(p.rows + (size_t)s * p.chunks + c);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const int s = i0 + i < p.k ? slot[i0 + i] : -1;
             if (s < 0 || s >= p.R) continue;
             const float w = weight[i0 + i];
@@ -893,7 +901,7 @@ size_t wf_expert_dispatch_workspace_bytes(int64_t T, int32_t topk, int32_t n_exp
     if (!disp_ok(T, topk, n_experts)) return 0;
     int run;
     const int n = disp_chunks(T * topk, &run);
-    return n > 1 ? (size_t)n * n_experts * 4 : 0;
+    return n > 1 ? (size_t)n * ((n_experts + 3) / 4 * 4) * 4 : 0;
 }
 
 int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32_t topk, int32_t n_experts,
@@ -907,11 +915,11 @@ int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32
     if (need && (!workspace || workspace_bytes < need))
         return fail(WF_E_ARG, "workspace too small (see wf_expert_dispatch_workspace_bytes)");
     if (misaligned(indices, indices_64 ? 8 : 4) || misaligned(offsets, 4) || misaligned(tokens, 4) ||
-        misaligned(slots, 4) || misaligned(workspace, 4))
-        return fail(WF_E_ARG, "misaligned pointer");
+        misaligned(slots, 4) || misaligned(workspace, 16))
+        return fail(WF_E_ARG, "misaligned pointer (indices to their size, the workspace to 16 bytes, the rest to 4)");
     DispArgs p;
     p.indices = indices; p.idx64 = indices_64 != 0; p.pairs = (int)(T * topk); p.k = topk; p.E = n_experts;
-    p.base = (int)expert_offset; p.hist = (int *)workspace; p.offsets = offsets; p.tokens = tokens; p.slots = slots;
+    p.row = (n_experts + 3) / 4 * 4; p.base = (int)expert_offset; p.hist = (int *)workspace; p.offsets = offsets; p.tokens = tokens; p.slots = slots;
     p.nchunks = disp_chunks(p.pairs, &p.run);
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e = cudaSuccess;
