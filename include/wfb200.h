@@ -370,7 +370,7 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
                         void *out, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Bytes of workspace for the call above (no initial value needed; 16-byte aligned): the listed
- * rows in expert order, R * K, when a row list has many rows per expert, else 0 (then the
+ * rows in expert order, R * K, when a row list has more than a few rows per expert, else 0 (then the
  * workspace may be NULL).  row_list: whether rows is given. */
 size_t wf_grouped_fp8_workspace_bytes(int32_t row_list, int64_t R, int32_t E, int64_t K);
 

@@ -301,3 +301,53 @@ def test_zero_rows_and_refusals():
         with pytest.raises(err):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+@pytest.mark.parametrize("per", [3, 200])
+def test_a_wait_that_runs_out_is_reported(kind, per):
+    """With the bound of device waits at 200 cycles a wait for a copy runs out: the call ends early and says so, and
+    the next call is not affected."""
+    from wanferenz_b200 import _lib as L
+    ops = _ops()
+    g = _gen(10, per)
+    E, N, K = 4, 512, 2048
+    a, a_s, w, w_s = _operands(g, E * per, E, N, K, kind, kind)
+    off = _offsets([per] * E)
+    want = ops.grouped_fp8_gemm(a, a_s, w, w_s, off)
+    ops.grouped_read_error()
+    try:
+        L.check(L.load().wf_set_wait_limit(200), "wf_set_wait_limit")
+        ops.grouped_fp8_gemm(a, a_s, w, w_s, off)
+        with pytest.raises(L.WfError) as e:
+            ops.grouped_read_error()
+        assert e.value.code == L.WF_E_TIMEOUT
+    finally:
+        L.load().wf_set_wait_limit(0)
+    assert torch.equal(want, ops.grouped_fp8_gemm(a, a_s, w, w_s, off))
+    ops.grouped_read_error()
+
+
+def test_views_off_a_16_byte_boundary():
+    """Inputs that start inside a 16-byte line are copied, an output that does is refused."""
+    ops = _ops()
+    g = _gen(11)
+    a, a_s, w, w_s = _operands(g, 24, 2, 256, 256, torch.float32, E8)
+    off = _offsets([9, 15])
+    want = ops.grouped_fp8_gemm(a, a_s, w, w_s, off)
+
+    def shifted(t):
+        s = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        s.copy_(t)
+        return s
+
+    got = ops.grouped_fp8_gemm(shifted(a), shifted(a_s), shifted(w), shifted(w_s), shifted(off))
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError):
+        ops.grouped_fp8_gemm(a, a_s, w, w_s, off, out=shifted(want))
+    x = torch.randn(5, 256, generator=g, device="cuda").bfloat16()
+    r, s = ops.rms_norm_quant(x, torch.ones(256, device="cuda"), residual=x), None
+    s = ops.rms_norm_quant(shifted(x), shifted(torch.ones(256, device="cuda")), residual=shifted(x))
+    assert torch.equal(r.q.view(torch.uint8), s.q.view(torch.uint8)) and torch.equal(r.s, s.s) and torch.equal(r.y, s.y)
+    slots = torch.arange(5, device="cuda").int().view(5, 1)
+    assert torch.equal(ops.expert_combine(shifted(x), shifted(slots), shared=shifted(x)), ops.expert_combine(x, slots, shared=x))

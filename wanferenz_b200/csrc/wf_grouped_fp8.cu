@@ -4,8 +4,8 @@
 //   for expert e and r in [offsets[e], offsets[e+1]), row(r) = rows[r] (or r)
 //
 // Weight rows are the M side of the MMA, tokens the N side: an expert's rows are cut
-// into tiles of equal width, a multiple of 32 up to 256, so a few rows cost a few
-// columns and nothing is padded to 128.  A pair of CTAs (cta_group::2) works on 256
+// into tiles of about equal width, multiples of 32 up to 256, so a few rows cost a few
+// columns and an expert pads to 32 rows once.  A pair of CTAs (cta_group::2) works on 256
 // weight rows: each holds 128 of them (one block of weight scales) and half of the
 // tokens in shared memory, and the products of its own 128 rows in its TMEM, so a
 // 256-wide tile moves 32 KB into each SM per 128-wide K step, half of what single
@@ -39,7 +39,15 @@ __device__ int g_err;  // error flags of the grouped products since the last wf_
 
 constexpr int MAX_E = 512;
 constexpr int SGRP = 8;                 // K steps per group of scales
-constexpr int FEW = 64;                 // rows per expert up to which tiles are narrow and row lists gathered in place
+// Rows per expert up to which tiles are narrow (32 experts of 2048 x 2048, rows in order, narrow
+// against wide tiles in us: e8m0 48 rows 27.8 / 34.1, 64 31.2 / 35.1, 96 40.2 / 36.8; f32 48 rows
+// 32.1 / 32.3, 64 37.0 / 33.9) ...
+constexpr int NARROW_E8 = 64, NARROW_F32 = 48;
+// ... and up to which a row list is gathered in place, by TMA copies of four rows, instead of
+// packed into expert order first (the same with e8m0 and narrow tiles: gathered 4 rows 28.1, 8 30.4,
+// 16 33.3, 32 40.0; packed 16 29.9, 32 30.3).  The TMA unit takes about 80 cycles for a four-row
+// copy, as long as for a box of 128 rows.
+constexpr int GATHER = 12;
 constexpr int W_PROD = 0, W_MMA = 1, WORKERS = 8;
 constexpr int SMEM_MAX = 232448;
 constexpr int TAB_BYTES = (3 * MAX_E + 4) * 4;  // per expert: first row, rows, first token tile
@@ -67,13 +75,19 @@ struct Plan {
     static_assert(E8 ? NACC * NT <= 256 && COL_SFB + 2 * SGRP * SFB <= 512 : NT == 64, "tensor memory");
 };
 
+// The bound of the waits on another role: a wait ends `cycles` after its first miss.  A bound lowered
+// by wf_set_wait_limit is kept by polling; try_wait may suspend the thread for longer.
+struct Bound {
+    long long cycles;
+    uint32_t poll;
+};
 struct Args {
     CUtensorMap tmW;     // weights [E*N, K], box 128 x 128
     CUtensorMap tmA[4];  // rows [M, K], boxes of 128, 64, 32 and 16 rows; the first of one row to gather
     const void *a_s, *w_s;
     const int *offsets, *rows;
     __nv_bfloat16 *out;
-    long long limit;
+    Bound limit;
     int M, R, E, N, K, a_f32, w_f32;
     int gather;          // the tensor map's rows are those of `rows`, else the product's own
 };
@@ -100,13 +114,26 @@ __device__ __forceinline__ uint32_t leader_addr(const void *p) {
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+__device__ __forceinline__ bool wait_once(uint64_t *bar, uint32_t parity, uint32_t poll) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "@q mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@!q mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(poll)
+        : "memory");
+    return ok != 0;
+}
 // Bounded wait; a wait that runs out sets the error flag and tells the CTA's other roles.
-__device__ __forceinline__ bool twait(uint64_t *bar, uint32_t parity, volatile int *abort, long long limit) {
-    if (mbar_try_wait(bar, parity)) return true;
+__device__ __forceinline__ bool twait(uint64_t *bar, uint32_t parity, volatile int *abort, const Bound &limit) {
+    if (wait_once(bar, parity, limit.poll)) return true;
     const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
+    while (!wait_once(bar, parity, limit.poll)) {
         if (*abort) return false;
-        if (clock64() - t0 > limit) {
+        if (clock64() - t0 > limit.cycles) {
             atomicOr(&g_err, kErrTimeout);
             *abort = 1;
             return false;
@@ -271,7 +298,7 @@ struct Walk {
     Table tab;
     int E, nn, step, e;
     long long i;
-    // Cuts an expert's rows into tiles of equal width (even: a multiple of 32) or of `fixed` rows.
+    // Cuts an expert's rows into tiles whose widths differ by 32 at most, or of `fixed` rows.
     __device__ bool next(Tile &t, int fixed = 0) {
         while (e < E && i >= (long long)tab.first[e + 1] * nn) ++e;
         if (e >= E) return false;
@@ -279,10 +306,16 @@ struct Walk {
         const int nt = tab.first[e + 1] - tab.first[e], c = tab.cnt[e];
         t.e = e;
         t.n0 = local % nn * 256;
-        t.width = fixed ? fixed : ((c + nt - 1) / nt + 31) / 32 * 32;  // cta_group::2 takes N in steps of 32
-        const int j = local / nn * t.width;
-        t.r0 = tab.lo[e] + j;
-        t.nrow = min(t.width, c - j);
+        const int j = local / nn;
+        int at = j * fixed;
+        t.width = fixed;
+        if (!fixed) {  // cta_group::2 takes N in steps of 32
+            const int units = (c + 31) / 32, each = units / nt, more = units - each * nt;
+            t.width = 32 * (each + (j < more));
+            at = 32 * (j * each + min(j, more));
+        }
+        t.r0 = tab.lo[e] + at;
+        t.nrow = min(t.width, c - at);
         i += step;
         return true;
     }
@@ -454,7 +487,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
                 }
             }
             if (leader) commit2(fin, 1);  // TMEM and the peer's operands go only when every MMA is done
-            twait(fin, 0, abort, kWaitLimitCycles);
+            twait(fin, 0, abort, Bound{kWaitLimitCycles, 0});
         }
     } else if (warp < L::SCALE0) {
         // (no role)
@@ -790,7 +823,7 @@ __global__ void __launch_bounds__(wide::THREADS, 1) k_grouped_f32_wide(const __g
                 }
             }
             if (leader) commit(fin);  // TMEM goes only when every MMA is done
-            twait(fin, 0, abort, kWaitLimitCycles);
+            twait(fin, 0, abort, Bound{kWaitLimitCycles, 0});
         }
     } else {
         // worker (q, half): the 32 tokens of TMEM lane quadrant q, 128 weight rows (one block of scales)
@@ -940,7 +973,7 @@ extern "C" {
 
 size_t wf_grouped_fp8_workspace_bytes(int32_t row_list, int64_t R, int32_t E, int64_t K) {
     if (R <= 0 || R > (1 << 30) || E <= 0 || E > wf::grp::MAX_E || K <= 0 || K > (1 << 20)) return 0;
-    return row_list && R > (int64_t)E * wf::grp::FEW ? (size_t)R * K : 0;
+    return row_list && R > (int64_t)E * wf::grp::GATHER ? (size_t)R * K : 0;
 }
 
 int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, const void *w, const void *w_s,
@@ -958,11 +991,7 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
         (a_scale_kind == WF_SCALE_F32 && (uintptr_t)a_s % 4) || (w_scale_kind == WF_SCALE_F32 && (uintptr_t)w_s % 4))
         return fail(WF_E_ARG, "a, w and out must be 16-byte aligned, f32 scales and row lists 4-byte");
     wf::grp::Args p;
-    // Many rows per expert: a copy of the listed rows in expert order, then whole boxes of it.  Few:
-    // four rows a copy straight from a.  The TMA unit takes about 80 cycles for a four-row copy, so up
-    // to 32 rows of a CTA (a tile of 64) hide behind the 128 weight rows of a K step (about 700 cycles of
-    // its share of HBM), and 128 take four times as long as their product.
-    const bool pack = rows && R > (int64_t)E * wf::grp::FEW;
+    const bool pack = rows && R > (int64_t)E * wf::grp::GATHER;
     if (pack) {
         if (!workspace || workspace_bytes < (size_t)R * K) return fail(WF_E_ARG, "workspace too small (see wf_grouped_fp8_workspace_bytes)");
         if ((uintptr_t)workspace % 16) return fail(WF_E_ARG, "workspace must be 16-byte aligned");
@@ -977,12 +1006,13 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
     }
     if (rc) return rc;
     p.a_s = a_s; p.w_s = w_s; p.offsets = offsets; p.rows = rows; p.out = (__nv_bfloat16 *)out;
-    p.limit = wf::host::wait_limit();
+    p.limit.cycles = wf::host::wait_limit();
+    p.limit.poll = p.limit.cycles < wf::kWaitLimitCycles;
     p.M = (int)M; p.R = (int)R; p.E = E; p.N = (int)N; p.K = (int)K;
     p.a_f32 = a_scale_kind == WF_SCALE_F32; p.w_f32 = w_scale_kind == WF_SCALE_F32;
     const int sms = wf::host::sm_count();
     if (sms <= 0) return fail(WF_E_CUDA, "no CUDA device");
-    const bool e8 = !p.a_f32 && !p.w_f32, few = R <= (int64_t)E * wf::grp::FEW;
+    const bool e8 = !p.a_f32 && !p.w_f32, few = R <= (int64_t)E * (e8 ? wf::grp::NARROW_E8 : wf::grp::NARROW_F32);
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e = cudaSuccess;
     if (pack) {

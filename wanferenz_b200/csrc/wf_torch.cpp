@@ -38,7 +38,8 @@ std::string shape_text(at::IntArrayRef s) {
     return r + (s.size() == 1 ? ",)" : ")");
 }
 
-// A CUDA tensor of one of the types (on `dev` when given), contiguous.
+// A CUDA tensor of one of the types (on `dev` when given), contiguous and 16-byte aligned: another
+// layout, or a view that starts off a 16-byte boundary, is copied first.
 at::Tensor tensor(PyObject *o, const char *name, std::initializer_list<ScalarType> types, const char *types_text,
                   const at::Device *dev = nullptr) {
     if (!THPVariable_Check(o)) raise(PyExc_TypeError, "%s must be a tensor, not %.80s", name, Py_TYPE(o)->tp_name);
@@ -49,7 +50,8 @@ at::Tensor tensor(PyObject *o, const char *name, std::initializer_list<ScalarTyp
     if (!ok) raise(PyExc_TypeError, "%s has dtype %s, expected %s", name, c10::toString(t.scalar_type()), types_text);
     if (dev && t.device() != *dev)
         raise(PyExc_ValueError, "%s is on %s, expected %s", name, t.device().str().c_str(), dev->str().c_str());
-    return t.is_contiguous() ? t : t.contiguous();
+    if (!t.is_contiguous()) return t.contiguous();
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t;
 }
 
 void want_shape(const at::Tensor &t, const char *name, at::IntArrayRef s) {
@@ -252,7 +254,7 @@ WF_ENTRY(grouped_fp8_gemm, 7) {
     } else {
         out = tensor(a[6], "out", {at::kBFloat16}, BF16, &dev);
         want_shape(out, "out", {r, n});
-        if (!out.is_same(THPVariable_Unpack(a[6]))) raise(PyExc_ValueError, "out must be contiguous");
+        if (!out.is_same(THPVariable_Unpack(a[6]))) raise(PyExc_ValueError, "out must be contiguous and 16-byte aligned");
     }
     if (r) {
         if (!m) raise(PyExc_ValueError, "a has no rows to take");
