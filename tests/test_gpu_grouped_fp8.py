@@ -351,3 +351,19 @@ def test_views_off_a_16_byte_boundary():
     assert torch.equal(r.q.view(torch.uint8), s.q.view(torch.uint8)) and torch.equal(r.s, s.s) and torch.equal(r.y, s.y)
     slots = torch.arange(5, device="cuda").int().view(5, 1)
     assert torch.equal(ops.expert_combine(shifted(x), shifted(slots), shared=shifted(x)), ops.expert_combine(x, slots, shared=x))
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+def test_offsets_past_32_bits(kind):
+    """An output of more than 2^31 elements, rows listed and packed: the last rows are as right as the first."""
+    ops = _ops()
+    g = _gen(12)
+    R, N, K = 600000, 4096, 128
+    a, a_s, w, w_s = _operands(g, 1000, 2, N, K, kind, kind)
+    rows = (torch.arange(R, device="cuda") % 1000).int()
+    off = torch.tensor([0, 599990, R], device="cuda").int()
+    out = ops.grouped_fp8_gemm(a, a_s, w, w_s, off, rows=rows)
+    few = ops.grouped_fp8_gemm(a, a_s, w[1:], w_s[1:], _offsets([10]), rows=rows[-10:].contiguous())
+    assert torch.equal(out[-10:], few)
+    part = torch.cat([torch.arange(40), torch.arange(599990 - 40, 599990)]).cuda()
+    _check(out[part], a, a_s, w[:1], w_s[:1], _offsets([80]), rows[part])

@@ -516,3 +516,47 @@ def test_route_topk_large_and_cancelling_biases():
     _check_route(logits, 8, bias, "sigmoid", 8, 4)
     _check_route(logits - 100, 8, None, "sqrtsoftplus")
     _check_route(logits - 95, 8, None, "sigmoid")
+
+
+def test_outputs_are_complete_before_the_next_product_reads_them():
+    """A norm's q is the weight operand of the framework's FP8 product at once, which reads weights ahead of its wait."""
+    ops = _ops()
+    g = _gen(42)
+    w = torch.ones(2048, device="cuda")
+    a = (torch.randn(4, 2048, generator=g, device="cuda") * 60).to(torch.float8_e4m3fn)
+    a_s = torch.ones(4, 16, device="cuda").to(E8)
+    b_s = torch.ones(32, 16, device="cuda").to(E8)
+    for k in range(20):
+        x = torch.randn(4096, 2048, generator=g, device="cuda").bfloat16()
+        res = torch.randn(4096, 2048, generator=g, device="cuda").bfloat16()
+        torch.cuda.synchronize()
+        r = ops.rms_norm_quant(x, w, residual=res, norm_out=False, scale_fmt="ue8m0", scale_dtype=E8)
+        c = ops.fp8_gemm(a, a_s, r.q, b_s)
+        torch.cuda.synchronize()
+        assert torch.equal(c, ops.fp8_gemm(a, a_s, r.q, b_s)), k
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows are as right as the first."""
+    ops = _ops()
+    T, D = 150000, 16384  # 2.46e9 elements
+    x = torch.ones(T, D, dtype=torch.bfloat16, device="cuda")
+    x[-1, ::2] = 3.0
+    r = ops.rms_norm_quant(x, torch.ones(D, device="cuda"), norm_out=True)
+    want = ops.rms_norm_quant(x[-1:].clone(), torch.ones(D, device="cuda"), norm_out=True)
+    for i, ref in ((0, None), (-1, want), (T - 2, None)):
+        if ref is None:
+            ref = ops.rms_norm_quant(x[i:i + 1 or None].clone(), torch.ones(D, device="cuda"), norm_out=True)
+        assert torch.equal(r.q[i].view(torch.uint8), ref.q[0].view(torch.uint8))
+        assert torch.equal(r.s[i], ref.s[0]) and torch.equal(r.y[i], ref.y[0])
+    slots = torch.tensor([[T - 1, 0], [T - 2, T - 1], [1, T]], device="cuda").int()
+    y = ops.expert_combine(x, slots)
+    assert torch.equal(y[0].float(), x[-1].float() + 1) and torch.equal(y[1], y[0]) and bool((y[2] == 1).all())
+    del r, x, want
+    T, E = 4300000, 512  # 2.2e9 logits
+    logits = torch.zeros(T, E, dtype=torch.bfloat16, device="cuda")
+    logits[-1, 300] = logits[-1, 17] = 1.0
+    logits[0, 5] = 2.0
+    w, i = ops.route_topk(logits, 2)
+    assert i[-1].tolist() == [17, 300] and i[0].tolist() == [5, 0] and i[T // 2].tolist() == [0, 1]
+    assert bool((w[1:].sum(-1) - 1).abs().max() < 1e-6)

@@ -373,7 +373,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
         fence_mbar_init();
     }
     if (warp == W_MMA) tmem_alloc2(tmem_base, 512);
-    pdl_launch_dependents();
     pdl_wait();
     const Table tab(base + L::OFF_TAB);
     tab.fill(p, NT);
@@ -761,7 +760,6 @@ __global__ void __launch_bounds__(wide::THREADS, 1) k_grouped_f32_wide(const __g
         fence_mbar_init();
     }
     if (warp == W_MMA) { tmem_alloc(tmem_base, 512); tmem_relinquish(); }
-    pdl_launch_dependents();
     pdl_wait();
     const Table tab(base + OFF_TAB);
     tab.fill(p, MT);
@@ -897,8 +895,8 @@ __global__ void __launch_bounds__(wide::THREADS, 1) k_grouped_f32_wide(const __g
 constexpr int PACK_STEP = 4 * 256;
 __global__ void __launch_bounds__(256) k_pack_rows(const uint4 *a, const int *rows, const int *offsets, uint4 *out, int E,
                                                    int M, int R, int chunks) {
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     // rows behind the last expert's are left out; the offsets need not rise
     int end = 0;
     for (int e = threadIdx.x; e <= E; e += 256) end = max(end, __ldg(offsets + e));

@@ -27,7 +27,10 @@ EncodeTiledFn encode_fn() noexcept;
 
 // Launches `kernel` so that it may start while the kernel before it on the stream drains
 // (programmatic dependent launch).  Every CTA of `kernel` executes griddepcontrol.wait before it
-// touches global memory, so the order of the stream holds for what it reads and writes.
+// touches global memory, so the order of the stream holds for what it reads and writes.  Only the
+// first kernel of an operator's two lets the next start early (griddepcontrol.launch_dependents),
+// behind its own wait, when all before it is done: the framework's products read their weights
+// ahead of their wait, so no kernel whose output a caller may pass on does.
 template <class... P, class... A>
 cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};

@@ -79,7 +79,6 @@ __global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __g
             }
         }
     };
-    pdl_launch_dependents();
     pdl_wait();
     if (blockIdx.x < p.T) load(blockIdx.x);
     int flip = 0;
@@ -521,7 +520,6 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS, N <= 8 ? 8 : 4) k_route_topk
     __shared__ uint32_t sm[ROUTE_WARPS][32 * N];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long t = (long long)blockIdx.x * ROUTE_WARPS + warp;
-    pdl_launch_dependents();
     pdl_wait();
     if (t >= p.T) return;
     float z[N], bias[N];
@@ -595,7 +593,7 @@ __device__ __forceinline__ void disp_load(const DispArgs &p, int i0, int hi, int
 __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_count(const __grid_constant__ DispArgs p) {
     __shared__ int cnt[DISP_MAX_E];
     pdl_wait();
-    pdl_launch_dependents();  // (after the wait: the placing kernel reads the indices without one)
+    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5;
     const int lo = min(p.pairs, (blockIdx.x * DISP_WARPS + warp) * p.run), hi = min(p.pairs, lo + p.run);
     int e[DISP_LANE];
@@ -620,7 +618,8 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid
     const int lo = min(p.pairs, (blockIdx.x * DISP_WARPS + warp) * p.run), hi = min(p.pairs, lo + p.run);
     const bool whole = hi - lo <= DISP_STEP;  // the run stays in registers
     int e[DISP_LANE], ahead[DISP_LANE];
-    pdl_launch_dependents();
+    // After the counting kernel, which lets this one start only when everything before it is done,
+    // the indices can be read at once.
     if (p.nchunks == 1) pdl_wait();
     disp_load(p, lo, hi, e);
     for (int x = lane; x < p.E; x += 32) cnt[warp][x] = 0;
@@ -743,7 +742,6 @@ __global__ void __launch_bounds__(256) k_combine(const __grid_constant__ CombArg
     __shared__ float weight[COMB_MAX_K];
     const size_t t = blockIdx.x;
     const int lane = threadIdx.x & 31;
-    pdl_launch_dependents();
     pdl_wait();
     if (threadIdx.x < 32) {
         const int s = lane < p.k ? p.slots[t * p.k + lane] : -1;
