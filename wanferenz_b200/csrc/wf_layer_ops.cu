@@ -198,6 +198,9 @@ __global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __g
 // sqrt(softplus) are screened in 32 bits first (route32); rows whose choice 32 bits
 // cannot settle, and softmax, take the 64-bit path (route64).  The chosen experts'
 // weights are in 64 bits on both.
+// Bound by instructions (about 1300 a token with 8 groups; the logits' bytes would take 1.4 us):
+// 8191 x 256, 8 groups, k = 8 takes 17 us.  All in 64 bits took 43, whole rows sent to route64
+// for one close call 28.
 // ---------------------------------------------------------------------------
 constexpr int ROUTE_MAX_E = 512, ROUTE_MAX_K = 16, ROUTE_MAX_G = 32;
 constexpr int ROUTE_WARPS = 4;
@@ -407,8 +410,8 @@ __device__ __noinline__ uint32_t groups64(const RouteArgs &p, long long t, const
 // is put in its place by the 64-bit values of the winners so far, one evaluation in all lanes at
 // once, and so is a choice of groups (0.1 % of rows of 8 groups).  Rows with NaN, +infinity or too
 // few experts and long runs of equal values are left to route64, which takes several times as
-// long (and a launch as long as its slowest row: settling rows here took 8191 x 256 in 8 groups
-// from 30 to 19 us).  Returns whether the row was settled; lane j < k has the expert of slot j.
+// long, and a launch takes as long as its slowest row.  Returns whether the row was settled;
+// lane j < k has the expert of slot j.
 template <int N>
 __device__ __forceinline__ bool route32(const RouteArgs &p, long long t, const float (&z)[N], const float (&bias)[N],
                                         uint32_t *sm, int &my_idx) {
@@ -483,23 +486,33 @@ __device__ __forceinline__ bool route32(const RouteArgs &p, long long t, const f
         for (int i = 0; i < N; ++i)
             if (!(kept >> ((lane + 32 * i) * p.magic >> 20) & 1)) key[i] = 0;  // (past E: 0 already)
     }
+    // each lane's keys in descending order (a bitonic network): a winner is the head of its lane
+#pragma unroll
+    for (int size = 2; size <= N; size <<= 1)
+#pragma unroll
+        for (int st = size >> 1; st > 0; st >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if ((i & st) == 0) {
+                    const uint32_t hi = max(key[i], key[i | st]), lo = min(key[i], key[i | st]);
+                    key[i] = (i & size) == 0 ? hi : lo;
+                    key[i | st] = (i & size) == 0 ? lo : hi;
+                }
     my_idx = -1;
     float last = 0.f, kth = 0.f;
     for (int j = 0; j < p.k + 8; ++j) {
-        uint32_t a = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) a = max(a, key[i]);
-        const uint32_t m = __reduce_max_sync(0xffffffffu, a);
+        const uint32_t m = __reduce_max_sync(0xffffffffu, key[0]);
         if (!m) return j >= p.k;
         const float v = value32(m);
         // the slots hold the k best so far: what is left cannot pass the k-th by its error
         if (j >= p.k && kth - v > gap0 + fmaxf(fabsf(kth), fabsf(v)) * 0x1p-17f) return true;
-        const int who = __ffs(__ballot_sync(0xffffffffu, a == m)) - 1;
+        const int who = __ffs(__ballot_sync(0xffffffffu, key[0] == m)) - 1;
         const int e = who + 32 * (int)(m & 15);
-        const uint32_t gone = lane == who ? m : 0u;
+        if (lane == who) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (key[i] == gone) key[i] = 0;
+            for (int i = 0; i + 1 < N; ++i) key[i] = key[i + 1];
+            key[N - 1] = 0;
+        }
         if (j == 0 || last - v > gap0 + fmaxf(fabsf(last), fabsf(v)) * 0x1p-17f) {
             if (lane == j) my_idx = e;
         } else {
@@ -516,7 +529,7 @@ __device__ __forceinline__ bool route32(const RouteArgs &p, long long t, const f
 }
 
 template <int N>  // experts per lane
-__global__ void __launch_bounds__(32 * ROUTE_WARPS, N <= 8 ? 8 : 4) k_route_topk(const __grid_constant__ RouteArgs p) {
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, N <= 8 ? 10 : 4) k_route_topk(const __grid_constant__ RouteArgs p) {
     __shared__ uint32_t sm[ROUTE_WARPS][32 * N];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long t = (long long)blockIdx.x * ROUTE_WARPS + warp;
