@@ -937,21 +937,16 @@ int tensor_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t K, uint
 // `nt` rows x 256 weight rows.
 template <void (*kernel)(const Args)>
 cudaError_t launch(const Args &p, int ctas, int nt, int threads, int smem, int sms, cudaStream_t st, int regs = 0) {
-    // once per device (the attribute is the function's, whichever thread sets it)
-    static std::atomic<uint64_t> ready{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    static std::atomic<uint64_t> ready[64];
+    cudaError_t e = host::allow_smem((const void *)kernel, 0, smem, ready);
     if (e != cudaSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (dev > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-        // a register split of more than the block is launched with would wait for ever
-        cudaFuncAttributes a;
-        e = cudaFuncGetAttributes(&a, kernel);
-        if (e != cudaSuccess) return e;
-        if (a.numRegs < regs) return cudaErrorInvalidConfiguration;
-        ready.fetch_or(bit, std::memory_order_relaxed);
+    if (regs) {  // a register split of more than the block is launched with would wait for ever
+        static const cudaFuncAttributes attr = [] {
+            cudaFuncAttributes a = {};
+            if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess) a.numRegs = 0;
+            return a;
+        }();
+        if (attr.numRegs < regs) return cudaErrorInvalidConfiguration;
     }
     const int64_t tiles = ((int64_t)p.R / nt + (p.E < p.R ? p.E : p.R)) * ((p.N + 255) / 256), most = sms / ctas;
     return host::launch_pdl(kernel, dim3(ctas * (unsigned)(tiles < most ? tiles : most)), threads, smem, st, p);

@@ -4,6 +4,9 @@
 
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
 
 namespace wf {
 namespace host {
@@ -24,6 +27,20 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 // cuTensorMapEncodeTiled through the runtime's driver entry point (NULL when unavailable).
 EncodeTiledFn encode_fn() noexcept;
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device: set once per device and
+// `which` (0..63, the caller's own number for the kernel; the attribute is the function's, whichever
+// thread sets it).
+inline cudaError_t allow_smem(const void *kernel, int which, size_t bytes, std::atomic<uint64_t> (&done)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << which;
+    if (dev < 64 && (done[dev].load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done[dev].fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // Launches `kernel` so that it may start while the kernel before it on the stream drains
 // (programmatic dependent launch).  Every CTA of `kernel` executes griddepcontrol.wait before it

@@ -37,11 +37,12 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
 //   power of two; q = e4m3(n / s)
 // The statistics are those of the rounded h, which is what the next layer reads
 // back.  q is taken from the 32-bit n, not from y: one rounding fewer.
-// A CTA walks over rows; a thread keeps its 8-column chunks in registers between the
-// sum of squares and the output, so every input is read once, and has the next row's
-// inputs on their way meanwhile.  A block of 128 columns is 16 neighbouring lanes.
-// Bound by HBM: 16384 x 4096 with residual and both outputs, 604 MB, takes 102 us, 5.9 TB/s
-// (one CTA per row, without the loads ahead: 114 us).
+// A CTA walks over rows.  A thread copies its own 8-column chunks of the rows ahead into
+// shared memory (cp.async, so no thread waits for another's copies), keeps a row in registers
+// between the sum of squares and the output, and reads every input once.  A block of 128
+// columns is 16 neighbouring lanes.
+// Bound by HBM: 16384 x 4096 with residual and both outputs, 604 MB, takes 96 us, 6.3 TB/s
+// (one CTA per row: 114 us; the next row in registers: 102 us, and 4.1 TB/s at D = 8192).
 // ---------------------------------------------------------------------------
 struct NormArgs {
     const uint4 *x, *res;
@@ -53,6 +54,7 @@ struct NormArgs {
     int chunks;  // D / 8
     long long T;
     int weight_bf16, ue8m0, s_f32;
+    int depth;   // rows of a CTA in flight, 2 or 3
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -61,37 +63,78 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// CTAs of 256 threads that an SM holds at once, by chunks per thread (registers).
-constexpr int norm_ctas(int ch) { return ch <= 1 ? 6 : ch <= 2 ? 4 : ch <= 4 ? 2 : 1; }
+__device__ __forceinline__ void copy_ahead(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Waits until at most depth - 1 of this thread's groups of copies are in flight.
+__device__ __forceinline__ void copies_left(int depth) {
+    if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+}
 
-template <int CH>
-__global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __grid_constant__ NormArgs p) {
-    __shared__ float parts[2][8];
+constexpr int NORM_THREADS = 512;  // at most
+
+template <int CH>  // chunks per thread
+__global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quant(const __grid_constant__ NormArgs p) {
+    extern __shared__ uint4 ahead[];  // [depth][x, residual][CH][threads]
+    __shared__ __align__(16) float parts[2][NORM_THREADS / 32];
     const int nt = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint4 nx[CH], nr[CH];
-    auto load = [&](long long t) {
+    const int slot_size = (p.res ? 2 : 1) * CH * nt;
+    if (threadIdx.x < 2 * (NORM_THREADS / 32)) parts[0][threadIdx.x] = 0.f;  // warps that a narrow block does not have
+    pdl_wait();
+    float w[CH][8];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int c = threadIdx.x + i * nt;
-            if (c < p.chunks) {
-                nx[i] = __ldg(p.x + t * p.chunks + c);
-                if (p.res) nr[i] = __ldg(p.res + t * p.chunks + c);
+    for (int i = 0; i < CH; ++i) {
+        const int c = threadIdx.x + i * nt;
+        if (c >= p.chunks) continue;
+        if (p.weight_bf16) {
+            const uint4 a = __ldg((const uint4 *)p.weight + c);
+            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = bf2(u[j]);
+                w[i][2 * j] = f.x;
+                w[i][2 * j + 1] = f.y;
+            }
+        } else {
+            const float4 a = __ldg((const float4 *)p.weight + 2 * c), b = __ldg((const float4 *)p.weight + 2 * c + 1);
+            w[i][0] = a.x; w[i][1] = a.y; w[i][2] = a.z; w[i][3] = a.w;
+            w[i][4] = b.x; w[i][5] = b.y; w[i][6] = b.z; w[i][7] = b.w;
+        }
+    }
+    auto fetch = [&](long long t, int slot) {
+        if (t < p.T) {
+            uint4 *dst = ahead + slot * slot_size + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int c = threadIdx.x + i * nt;
+                if (c < p.chunks) {
+                    copy_ahead(dst + i * nt, p.x + t * p.chunks + c);
+                    if (p.res) copy_ahead(dst + (CH + i) * nt, p.res + t * p.chunks + c);
+                }
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    pdl_wait();
-    if (blockIdx.x < p.T) load(blockIdx.x);
-    int flip = 0;
+    for (int d = 0; d + 1 < p.depth; ++d) fetch(blockIdx.x + (long long)d * gridDim.x, d);
+    __syncthreads();
+    int flip = 0, slot = 0;
     for (long long t = blockIdx.x; t < p.T; t += gridDim.x, flip ^= 1) {
         const size_t row = (size_t)t * p.chunks;
         float *part = parts[flip];
+        const int last = slot == 0 ? p.depth - 1 : slot - 1;  // the slot that the row before this one left
+        fetch(t + (long long)(p.depth - 1) * gridDim.x, last);
+        copies_left(p.depth);
+        const uint4 *src = ahead + slot * slot_size + threadIdx.x;
+        if (++slot == p.depth) slot = 0;
         float v[CH][8];
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int c = threadIdx.x + i * nt;
             if (c < p.chunks) {
-                const uint32_t u[4] = {nx[i].x, nx[i].y, nx[i].z, nx[i].w};
+                const uint4 a = src[i * nt];
+                const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float2 f = bf2(u[j]);
@@ -99,11 +142,12 @@ __global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __g
                     v[i][2 * j + 1] = f.y;
                 }
                 if (p.res) {
-                    const uint32_t w[4] = {nr[i].x, nr[i].y, nr[i].z, nr[i].w};
+                    const uint4 b = src[(CH + i) * nt];
+                    const uint32_t r4[4] = {b.x, b.y, b.z, b.w};
                     uint32_t o[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float2 f = bf2(w[j]);
+                        const float2 f = bf2(r4[j]);
                         o[j] = pack_bf2(v[i][2 * j] + f.x, v[i][2 * j + 1] + f.y);
                         const float2 r = bf2(o[j]);
                         v[i][2 * j] = r.x;
@@ -115,13 +159,16 @@ __global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __g
                 for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
             }
         }
-        if (t + gridDim.x < p.T) load(t + gridDim.x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (lane == 0) part[warp] = ss;
         __syncthreads();
         ss = 0.f;
-        for (int w = 0; w < nt / 32; ++w) ss += part[w];
+#pragma unroll
+        for (int j = 0; j < NORM_THREADS / 32; j += 4) {
+            const float4 f = *reinterpret_cast<const float4 *>(part + j);
+            ss += (f.x + f.y) + (f.z + f.w);
+        }
         const float rstd = rsqrtf(ss * p.inv_d + p.eps);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -129,24 +176,9 @@ __global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __g
             const bool on = c < p.chunks;  // whole groups of 16 lanes: chunks is a multiple of 16
             float amax = 0.f;
             if (on) {
-                float w[8];
-                if (p.weight_bf16) {
-                    const uint4 a = __ldg((const uint4 *)p.weight + c);
-                    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 f = bf2(u[j]);
-                        w[2 * j] = f.x;
-                        w[2 * j + 1] = f.y;
-                    }
-                } else {
-                    const float4 a = __ldg((const float4 *)p.weight + 2 * c), b = __ldg((const float4 *)p.weight + 2 * c + 1);
-                    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-                    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-                }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    v[i][j] = v[i][j] * rstd * w[j];
+                    v[i][j] = v[i][j] * rstd * w[i][j];
                     amax = max_nan(amax, fabsf(v[i][j]));
                 }
             }
@@ -161,15 +193,13 @@ __global__ void __launch_bounds__(256, norm_ctas(CH)) k_rms_norm_quant(const __g
                 byte = s < CUDART_INF_F ? (b + 0x7fffffu) >> 23 : 0xffu;
                 s = byte < 0xffu ? __uint_as_float(byte << 23) : CUDART_NAN_F;
             }
-            uint32_t lo, hi;
-            if (p.ue8m0) {
-                const float inv = 1.0f / s;  // exact
-                lo = f32x2_to_e4m3x2(v[i][0] * inv, v[i][1] * inv) | (uint32_t)f32x2_to_e4m3x2(v[i][2] * inv, v[i][3] * inv) << 16;
-                hi = f32x2_to_e4m3x2(v[i][4] * inv, v[i][5] * inv) | (uint32_t)f32x2_to_e4m3x2(v[i][6] * inv, v[i][7] * inv) << 16;
-            } else {
-                lo = f32x2_to_e4m3x2(v[i][0] / s, v[i][1] / s) | (uint32_t)f32x2_to_e4m3x2(v[i][2] / s, v[i][3] / s) << 16;
-                hi = f32x2_to_e4m3x2(v[i][4] / s, v[i][5] / s) | (uint32_t)f32x2_to_e4m3x2(v[i][6] / s, v[i][7] / s) << 16;
-            }
+            // n * (1 / s): exact for a power of two (below 2^120, as n is finite), else within an ulp
+            // and a half of n / s
+            const float inv = !p.ue8m0 ? __frcp_rn(s) : byte < 0xffu ? __uint_as_float((254u - byte) << 23) : CUDART_NAN_F;
+            const uint32_t lo = f32x2_to_e4m3x2(v[i][0] * inv, v[i][1] * inv) |
+                                (uint32_t)f32x2_to_e4m3x2(v[i][2] * inv, v[i][3] * inv) << 16;
+            const uint32_t hi = f32x2_to_e4m3x2(v[i][4] * inv, v[i][5] * inv) |
+                                (uint32_t)f32x2_to_e4m3x2(v[i][6] * inv, v[i][7] * inv) << 16;
             p.q[row + c] = make_uint2(lo, hi);
             if (p.y)
                 p.y[row + c] = make_uint4(pack_bf2(v[i][0], v[i][1]), pack_bf2(v[i][2], v[i][3]),
@@ -817,6 +847,8 @@ __global__ void __launch_bounds__(256) k_combine(const __grid_constant__ CombArg
     }
 }
 
+std::atomic<uint64_t> norm_ready[64];  // devices on which a variant may use its shared memory
+
 int launched(cudaError_t e, const char *what) { return e == cudaSuccess ? WF_OK : cuda_fail(e, what); }
 
 bool misaligned(const void *p, uintptr_t to) { return (uintptr_t)p % to != 0; }
@@ -845,16 +877,27 @@ int wf_rms_norm_quant(const void *x, const void *residual, const void *weight, i
     p.y = (uint4 *)y; p.h = (uint4 *)h; p.q = (uint2 *)q; p.s = s;
     p.eps = eps; p.inv_d = 1.0f / (float)D; p.chunks = (int)(D / 8); p.T = T;
     p.weight_bf16 = weight_bf16 != 0; p.ue8m0 = ue8m0 != 0; p.s_f32 = scale_kind == WF_SCALE_F32;
-    const int ch = (p.chunks + 255) / 256;
-    const int nt = ch > 1 ? 256 : (p.chunks + 31) / 32 * 32;
     const int sms = wf::host::sm_count();
     if (sms <= 0) return fail(WF_E_CUDA, "no CUDA device");
-    const int ct = ch <= 2 ? ch : ch <= 4 ? 4 : 8;
-    const int per_sm = ct > 1 ? norm_ctas(ct) : norm_ctas(1) * 256 / nt < 32 ? norm_ctas(1) * 256 / nt : 32;
-    const int64_t most = (int64_t)sms * per_sm;
+    // Threads: one, two or four chunks each, the fewest that hold a row in a block.  CTAs: reads and
+    // writes together run best with few rows open at a time (with residual and both outputs, 2, 3 and
+    // 4 CTAs on an SM: D = 4096 6.4, 5.3 and 5.2 TB/s; D = 2048 5.3, 6.2 and 5.8); without the
+    // residual the instructions count and more threads help (D = 4096 4.2, 5.0 and 5.3 TB/s).
+    const int ch = p.chunks <= 256 ? 1 : p.chunks <= 1024 ? 2 : 4;
+    const int nt = ((p.chunks + ch - 1) / ch + 31) / 32 * 32;
+    const int threads = ch == 4 ? 512 : !residual ? 1024 : ch == 2 ? 704 : 768;
+    const int ctas = threads / nt < 32 ? threads / nt : 32;
+    const int64_t most = (int64_t)sms * ctas;
     const dim3 g((unsigned)(T < most ? T : most));
-    auto k = ct == 1 ? k_rms_norm_quant<1> : ct == 2 ? k_rms_norm_quant<2> : ct == 4 ? k_rms_norm_quant<4> : k_rms_norm_quant<8>;
-    return launched(wf::host::launch_pdl(k, g, nt, 0, (cudaStream_t)stream, p), "rms_norm_quant launch");
+    p.depth = T <= most || ch == 4 || (residual && ch == 1) ? 2 : 3;
+    const int room = 128 << 10;  // two rows of 16384 with their residuals
+    const size_t smem = (size_t)p.depth * (residual ? 2 : 1) * ch * nt * 16;
+    auto k = ch == 1 ? k_rms_norm_quant<1> : ch == 2 ? k_rms_norm_quant<2> : k_rms_norm_quant<4>;
+    if (smem > 47 << 10) {  // (the static arrays count too)
+        const cudaError_t e = wf::host::allow_smem((const void *)k, ch, room, norm_ready);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(rms_norm_quant)");
+    }
+    return launched(wf::host::launch_pdl(k, g, nt, smem, (cudaStream_t)stream, p), "rms_norm_quant launch");
 }
 
 int wf_route_topk(const void *logits, int32_t logits_bf16, const float *bias, int64_t T, int32_t E, int32_t topk,
