@@ -560,3 +560,17 @@ def test_offsets_past_32_bits():
     w, i = ops.route_topk(logits, 2)
     assert i[-1].tolist() == [17, 300] and i[0].tolist() == [5, 0] and i[T // 2].tolist() == [0, 1]
     assert bool((w[1:].sum(-1) - 1).abs().max() < 1e-6)
+
+
+def test_rms_norm_quant_overflowing_block():
+    """A norm past the largest float: its block's scale is infinite (e8m0: NaN), its finite values become 0 (NaN)."""
+    x = torch.zeros(1, 256, dtype=torch.bfloat16, device="cuda")
+    x[0, 0], x[0, 1], x[0, 130] = 16.0, 1.0, 1.0
+    w = torch.ones(256, device="cuda")
+    w[0] = 3e38
+    r = _ops().rms_norm_quant(x, w)
+    assert float(r.s[0, 0]) == float("inf") and bool(r.y[0, 0].isinf())
+    assert bool(r.q[0, 0].float().isnan()) and bool((r.q[0, 1:128].float() == 0).all())
+    assert float(r.q[0, 130].float()) == 448.0
+    e = _ops().rms_norm_quant(x, w, scale_fmt="ue8m0", scale_dtype=E8)
+    assert bool(e.s[0, 0].float().isnan()) and bool(e.q[0, :128].float().isnan().all()) and not bool(e.s[0, 1].float().isnan())

@@ -193,13 +193,19 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
                 byte = s < CUDART_INF_F ? (b + 0x7fffffu) >> 23 : 0xffu;
                 s = byte < 0xffu ? __uint_as_float(byte << 23) : CUDART_NAN_F;
             }
-            // n * (1 / s): exact for a power of two (below 2^120, as n is finite), else within an ulp
-            // and a half of n / s
+            // n / s: exact by the reciprocal of a power of two (below 2^120, as n is finite); else the
+            // product with the rounded reciprocal is put right by its remainder (0 for an infinite s)
             const float inv = !p.ue8m0 ? __frcp_rn(s) : byte < 0xffu ? __uint_as_float((254u - byte) << 23) : CUDART_NAN_F;
-            const uint32_t lo = f32x2_to_e4m3x2(v[i][0] * inv, v[i][1] * inv) |
-                                (uint32_t)f32x2_to_e4m3x2(v[i][2] * inv, v[i][3] * inv) << 16;
-            const uint32_t hi = f32x2_to_e4m3x2(v[i][4] * inv, v[i][5] * inv) |
-                                (uint32_t)f32x2_to_e4m3x2(v[i][6] * inv, v[i][7] * inv) << 16;
+            float u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = v[i][j] * inv;
+            if (!p.ue8m0) {
+                const float den = s < CUDART_INF_F ? s : 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] = fmaf(fmaf(-u[j], den, v[i][j]), inv, u[j]);
+            }
+            const uint32_t lo = f32x2_to_e4m3x2(u[0], u[1]) | (uint32_t)f32x2_to_e4m3x2(u[2], u[3]) << 16;
+            const uint32_t hi = f32x2_to_e4m3x2(u[4], u[5]) | (uint32_t)f32x2_to_e4m3x2(u[6], u[7]) << 16;
             p.q[row + c] = make_uint2(lo, hi);
             if (p.y)
                 p.y[row + c] = make_uint4(pack_bf2(v[i][0], v[i][1]), pack_bf2(v[i][2], v[i][3]),
