@@ -28,6 +28,24 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+// Two 32-bit operations in one instruction: (a0, a1) * (b0, b1) and + (c0, c1).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 r, a, b;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
 // ---------------------------------------------------------------------------
 // RMS norm + residual + E4M3 output
 //   h = bf16(x + residual)          (the residual stream; x itself without one)
@@ -82,7 +100,7 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
     const int slot_size = (p.res ? 2 : 1) * CH * nt;
     if (threadIdx.x < 2 * (NORM_THREADS / 32)) parts[0][threadIdx.x] = 0.f;  // warps that a narrow block does not have
     pdl_wait();
-    float w[CH][8];
+    float2 w[CH][4];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int c = threadIdx.x + i * nt;
@@ -91,15 +109,11 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
             const uint4 a = __ldg((const uint4 *)p.weight + c);
             const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = bf2(u[j]);
-                w[i][2 * j] = f.x;
-                w[i][2 * j + 1] = f.y;
-            }
+            for (int j = 0; j < 4; ++j) w[i][j] = bf2(u[j]);
         } else {
             const float4 a = __ldg((const float4 *)p.weight + 2 * c), b = __ldg((const float4 *)p.weight + 2 * c + 1);
-            w[i][0] = a.x; w[i][1] = a.y; w[i][2] = a.z; w[i][3] = a.w;
-            w[i][4] = b.x; w[i][5] = b.y; w[i][6] = b.z; w[i][7] = b.w;
+            w[i][0] = make_float2(a.x, a.y); w[i][1] = make_float2(a.z, a.w);
+            w[i][2] = make_float2(b.x, b.y); w[i][3] = make_float2(b.z, b.w);
         }
     }
     auto fetch = [&](long long t, int slot) {
@@ -127,8 +141,7 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
         copies_left(p.depth);
         const uint4 *src = ahead + slot * slot_size + threadIdx.x;
         if (++slot == p.depth) slot = 0;
-        float v[CH][8];
-        float ss = 0.f;
+        float2 v[CH][4], sq = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int c = threadIdx.x + i * nt;
@@ -136,11 +149,7 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
                 const uint4 a = src[i * nt];
                 const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = bf2(u[j]);
-                    v[i][2 * j] = f.x;
-                    v[i][2 * j + 1] = f.y;
-                }
+                for (int j = 0; j < 4; ++j) v[i][j] = bf2(u[j]);
                 if (p.res) {
                     const uint4 b = src[(CH + i) * nt];
                     const uint32_t r4[4] = {b.x, b.y, b.z, b.w};
@@ -148,17 +157,16 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 f = bf2(r4[j]);
-                        o[j] = pack_bf2(v[i][2 * j] + f.x, v[i][2 * j + 1] + f.y);
-                        const float2 r = bf2(o[j]);
-                        v[i][2 * j] = r.x;
-                        v[i][2 * j + 1] = r.y;
+                        o[j] = pack_bf2(v[i][j].x + f.x, v[i][j].y + f.y);
+                        v[i][j] = bf2(o[j]);
                     }
                     p.h[row + c] = make_uint4(o[0], o[1], o[2], o[3]);
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+                for (int j = 0; j < 4; ++j) sq = fma2(v[i][j], v[i][j], sq);
             }
         }
+        float ss = sq.x + sq.y;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (lane == 0) part[warp] = ss;
@@ -177,9 +185,9 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
             float amax = 0.f;
             if (on) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] = v[i][j] * rstd * w[i][j];
-                    amax = max_nan(amax, fabsf(v[i][j]));
+                for (int j = 0; j < 4; ++j) {
+                    v[i][j] = mul2(mul2(v[i][j], make_float2(rstd, rstd)), w[i][j]);
+                    amax = max_nan(amax, max_nan(fabsf(v[i][j].x), fabsf(v[i][j].y)));
                 }
             }
 #pragma unroll
@@ -196,20 +204,21 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
             // n / s: exact by the reciprocal of a power of two (below 2^120, as n is finite); else the
             // product with the rounded reciprocal is put right by its remainder (0 for an infinite s)
             const float inv = !p.ue8m0 ? __frcp_rn(s) : byte < 0xffu ? __uint_as_float((254u - byte) << 23) : CUDART_NAN_F;
-            float u[8];
+            float2 u[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) u[j] = v[i][j] * inv;
+            for (int j = 0; j < 4; ++j) u[j] = mul2(v[i][j], make_float2(inv, inv));
             if (!p.ue8m0) {
-                const float den = s < CUDART_INF_F ? s : 0.f;
+                const float den = s < CUDART_INF_F ? -s : 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) u[j] = fmaf(fmaf(-u[j], den, v[i][j]), inv, u[j]);
+                for (int j = 0; j < 4; ++j)
+                    u[j] = fma2(fma2(u[j], make_float2(den, den), v[i][j]), make_float2(inv, inv), u[j]);
             }
-            const uint32_t lo = f32x2_to_e4m3x2(u[0], u[1]) | (uint32_t)f32x2_to_e4m3x2(u[2], u[3]) << 16;
-            const uint32_t hi = f32x2_to_e4m3x2(u[4], u[5]) | (uint32_t)f32x2_to_e4m3x2(u[6], u[7]) << 16;
+            const uint32_t lo = f32x2_to_e4m3x2(u[0].x, u[0].y) | (uint32_t)f32x2_to_e4m3x2(u[1].x, u[1].y) << 16;
+            const uint32_t hi = f32x2_to_e4m3x2(u[2].x, u[2].y) | (uint32_t)f32x2_to_e4m3x2(u[3].x, u[3].y) << 16;
             p.q[row + c] = make_uint2(lo, hi);
             if (p.y)
-                p.y[row + c] = make_uint4(pack_bf2(v[i][0], v[i][1]), pack_bf2(v[i][2], v[i][3]),
-                                          pack_bf2(v[i][4], v[i][5]), pack_bf2(v[i][6], v[i][7]));
+                p.y[row + c] = make_uint4(pack_bf2(v[i][0].x, v[i][0].y), pack_bf2(v[i][1].x, v[i][1].y),
+                                          pack_bf2(v[i][2].x, v[i][2].y), pack_bf2(v[i][3].x, v[i][3].y));
             if ((lane & 15) == 0) {
                 const size_t at = (row + c) >> 4;
                 if (p.s_f32) ((float *)p.s)[at] = s;
