@@ -367,3 +367,17 @@ def test_offsets_past_32_bits(kind):
     assert torch.equal(out[-10:], few)
     part = torch.cat([torch.arange(40), torch.arange(599990 - 40, 599990)]).cuda()
     _check(out[part], a, a_s, w[:1], w_s[:1], _offsets([80]), rows[part])
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+def test_offsets_that_give_every_expert_all_rows(kind):
+    """Offsets that fall again and again: every second expert owns all rows; the call stays in bounds, and with equal
+    weights it does not matter which expert writes last."""
+    ops = _ops()
+    g = _gen(13)
+    a, a_s, w, w_s = _operands(g, 3000, 1, 128, 128, kind, kind)
+    E = 512
+    off = torch.tensor([0, 3000], device="cuda").repeat(E // 2 + 1)[:E + 1].int()
+    out = ops.grouped_fp8_gemm(a, a_s, w.view(torch.uint8).expand(E, 128, 128).contiguous().view(w.dtype),
+                               w_s.float().expand(E, 1, 1).contiguous().to(kind), off)
+    _check(out, a, a_s, w, w_s, _offsets([3000]), None)

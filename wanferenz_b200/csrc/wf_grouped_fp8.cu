@@ -19,6 +19,12 @@
 // (k_grouped_f32_wide): a token per TMEM lane, so that a thread's scale is one register.
 // (A scale per column comes from shared memory, 4 bytes a lane and column whether the
 // lanes read the same ones or not: 131 KB a K step, as many cycles as the whole product.)
+//
+// Measured on a B200.  Few rows per expert, bound by the weights' stream (5.5 TB/s while it
+// runs): 96 rows over 64 experts of 2048 x 2048, e8m0, 41 us (floor 32); 1536 rows over 64 of
+// 2048 x 1024, f32, 33.7 us (21.7).  Many, bound by the tensor cores and by power: one expert of
+// 16384 rows, 4096 x 4096, e8m0, 3.05 PFLOP/s in a burst, 2.4 sustained under the 1 kW cap; 16386
+// rows over 32 of these experts 256 us in a burst (174), 336 sustained; with f32 scales 390.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -50,7 +56,7 @@ constexpr int NARROW_E8 = 64, NARROW_F32 = 48;
 constexpr int GATHER = 12;
 constexpr int W_PROD = 0, W_MMA = 1, WORKERS = 8;
 constexpr int SMEM_MAX = 232448;
-constexpr int TAB_BYTES = (3 * MAX_E + 4) * 4;  // per expert: first row, rows, first token tile
+constexpr int TAB_BYTES = 2 * MAX_E * 4 + (MAX_E + 1) * 8;  // per expert: first row, rows, first token tile
 
 // NT: tokens per tile, at most.  Narrow tiles, for few rows per expert, leave room for ten stages and
 // for accumulators ahead of the workers: there the weights' stream from HBM is all that counts, and
@@ -257,10 +263,12 @@ struct Tile {
 };
 
 // Every expert's rows, clamped to the R rows there are, and its first token tile, in shared memory.
+// (Tiles are counted in 64 bits: offsets that fall again may give every expert all the rows.)
 struct Table {
-    int *lo, *cnt, *first;
+    int *lo, *cnt;
+    long long *first;
     __device__ explicit Table(uint8_t *at)
-        : lo(reinterpret_cast<int *>(at)), cnt(lo + MAX_E), first(cnt + MAX_E) {}
+        : lo(reinterpret_cast<int *>(at)), cnt(lo + MAX_E), first(reinterpret_cast<long long *>(cnt + MAX_E)) {}
     // By all threads; complete for the caller's next barrier.
     __device__ void fill(const Args &p, int nt) const {
         for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
@@ -271,17 +279,17 @@ struct Table {
         __syncthreads();
         if (threadIdx.x >= 32) return;
         const int lane = threadIdx.x;
-        int sum = 0, own[MAX_E / 32];
+        long long sum = 0, own[MAX_E / 32];
 #pragma unroll
         for (int j = 0; j < MAX_E / 32; ++j) {
             const int e = lane * (MAX_E / 32) + j;
             own[j] = sum;
             if (e < p.E) sum += (cnt[e] + nt - 1) / nt;
         }
-        int incl = sum;
+        long long incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            const long long v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
 #pragma unroll
@@ -300,10 +308,10 @@ struct Walk {
     long long i;
     // Cuts an expert's rows into tiles whose widths differ by 32 at most, or of `fixed` rows.
     __device__ bool next(Tile &t, int fixed = 0) {
-        while (e < E && i >= (long long)tab.first[e + 1] * nn) ++e;
+        while (e < E && i >= tab.first[e + 1] * nn) ++e;
         if (e >= E) return false;
-        const int local = (int)(i - (long long)tab.first[e] * nn);
-        const int nt = tab.first[e + 1] - tab.first[e], c = tab.cnt[e];
+        const int local = (int)(i - tab.first[e] * nn);
+        const int nt = (int)(tab.first[e + 1] - tab.first[e]), c = tab.cnt[e];
         t.e = e;
         t.n0 = local % nn * 256;
         const int j = local / nn;
