@@ -381,3 +381,47 @@ def test_offsets_that_give_every_expert_all_rows(kind):
     out = ops.grouped_fp8_gemm(a, a_s, w.view(torch.uint8).expand(E, 128, 128).contiguous().view(w.dtype),
                                w_s.float().expand(E, 1, 1).contiguous().to(kind), off)
     _check(out, a, a_s, w, w_s, _offsets([3000]), None)
+
+
+def test_two_streams_and_threads_at_once():
+    """Layers running at the same time on two streams, from two host threads, do not touch one another."""
+    import threading
+
+    g = _gen(14)
+    p = [_layer_params(g, 16, 512, 256) for _ in range(2)]
+    x = [torch.randn(T, 512, generator=g, device="cuda").bfloat16() for T in (3, 900)]
+    res = [torch.randn(T, 512, generator=g, device="cuda").bfloat16() for T in (3, 900)]
+    want = [_layer(x[i], res[i], p[i], 4)[0] for i in range(2)]
+    torch.cuda.synchronize()
+    got, bad = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i].append(_layer(x[i], res[i], p[i], 4)[0])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 (reported by the main thread)
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+    for i in range(2):
+        assert len(got[i]) == 20 and all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_inference_mode_and_parameters():
+    """Weights that are parameters, and calls inside inference mode, are taken as they are."""
+    g = _gen(15)
+    ops = _ops()
+    x = torch.randn(5, 256, generator=g, device="cuda").bfloat16()
+    w = torch.nn.Parameter(torch.rand(256, generator=g, device="cuda"))
+    want = ops.rms_norm_quant(x, w.detach())
+    with torch.inference_mode():
+        got = ops.rms_norm_quant(x, w)
+    assert torch.equal(want.y, got.y) and torch.equal(want.s, got.s) and not want.y.requires_grad
+    assert torch.equal(ops.rms_norm_quant(x, w).y, want.y)

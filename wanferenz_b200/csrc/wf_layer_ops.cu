@@ -59,7 +59,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 // shared memory (cp.async, so no thread waits for another's copies), keeps a row in registers
 // between the sum of squares and the output, and reads every input once.  A block of 128
 // columns is 16 neighbouring lanes.
-// Bound by HBM: 16384 x 4096 with residual and both outputs, 604 MB, takes 96 us, 6.3 TB/s
+// Bound by HBM: 16384 x 4096 with residual and both outputs, 604 MB, takes 94 to 102 us, 6 TB/s
 // (one CTA per row: 114 us; the next row in registers: 102 us, and 4.1 TB/s at D = 8192).
 // ---------------------------------------------------------------------------
 struct NormArgs {

@@ -20,7 +20,7 @@ way from the residual stream through the experts' products and back:
 * ``expert_combine(rows, slots, weights)``      the experts' rows back in token order
 
 These run on their tensors' device (which need not be the current one) and on its
-current stream, and keep nothing between calls.
+current stream, keep nothing between calls, and have no gradients.
 
 All tensors must be CUDA tensors; there is no CPU path.  Outputs are bf16,
 as the reference's are under the model's bf16 default dtype.
