@@ -900,32 +900,38 @@ __global__ void __launch_bounds__(wide::THREADS, 1) k_grouped_f32_wide(const __g
 }
 
 // The listed rows of a in the product's order (rows that do not exist: row 0, their results are zeroed).
-constexpr int PACK_STEP = 4 * 256;
-__global__ void __launch_bounds__(256) k_pack_rows(const uint4 *a, const int *rows, const int *offsets, uint4 *out, int E,
-                                                   int M, int R, int chunks) {
+// A warp per row, eight 16-byte pieces a lane in flight.
+constexpr int PACK_WARPS = 8;
+__global__ void __launch_bounds__(32 * PACK_WARPS) k_pack_rows(const uint4 *a, const int *rows, const int *offsets, uint4 *out,
+                                                               int E, int M, int R, int chunks) {
     pdl_wait();
     pdl_launch_dependents();
     // rows behind the last expert's are left out; the offsets need not rise
     int end = 0;
-    for (int e = threadIdx.x; e <= E; e += 256) end = max(end, __ldg(offsets + e));
-    __shared__ int ends[8];
+    for (int e = threadIdx.x; e <= E; e += 32 * PACK_WARPS) end = max(end, __ldg(offsets + e));
+    __shared__ int ends[PACK_WARPS];
     end = __reduce_max_sync(0xffffffffu, end);
-    if (threadIdx.x % 32 == 0) ends[threadIdx.x / 32] = end;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) ends[warp] = end;
+    const long long r0 = (long long)blockIdx.x * PACK_WARPS + warp, step = (long long)gridDim.x * PACK_WARPS;
+    int s = r0 < R ? __ldg(rows + r0) : 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) end = max(end, ends[w]);
-    const long long n = (long long)min(end, R) * chunks;
-    for (long long i0 = (long long)blockIdx.x * PACK_STEP + threadIdx.x; i0 < n; i0 += (long long)gridDim.x * PACK_STEP) {
-        uint4 v[4];
+    for (int w = 0; w < PACK_WARPS; ++w) end = max(end, ends[w]);
+    end = min(end, R);
+    for (long long r = r0; r < end; r += step) {
+        const uint4 *src = a + (size_t)(s >= 0 && s < M ? s : 0) * chunks;
+        uint4 *dst = out + r * chunks;
+        if (r + step < end) s = __ldg(rows + r + step);
+        for (int c0 = lane; c0 < chunks; c0 += 256) {
+            uint4 v[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long long i = min(i0 + 256 * j, n - 1);
-            const int r = (int)(i / chunks), s = __ldg(rows + r);
-            v[j] = __ldg(a + (size_t)(s >= 0 && s < M ? s : 0) * chunks + (i - (long long)r * chunks));
+            for (int j = 0; j < 8; ++j)
+                if (c0 + 32 * j < chunks) v[j] = __ldg(src + c0 + 32 * j);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + 32 * j < chunks) dst[c0 + 32 * j] = v[j];
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i0 + 256 * j < n) out[i0 + 256 * j] = v[j];
     }
 }
 
@@ -1017,9 +1023,10 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e = cudaSuccess;
     if (pack) {
-        const int64_t steps = R * (K / 16) / wf::grp::PACK_STEP + 1;
-        e = wf::host::launch_pdl(wf::grp::k_pack_rows, dim3((unsigned)(steps < 8 * sms ? steps : 8 * sms)), 256, 0, st,
-                                 (const uint4 *)a, rows, offsets, (uint4 *)workspace, (int)E, (int)M, (int)R, (int)(K / 16));
+        const int64_t ctas = (R + wf::grp::PACK_WARPS - 1) / wf::grp::PACK_WARPS, most = 16 * (int64_t)sms;
+        e = wf::host::launch_pdl(wf::grp::k_pack_rows, dim3((unsigned)(ctas < most ? ctas : most)), 32 * wf::grp::PACK_WARPS, 0,
+                                 st, (const uint4 *)a, rows, offsets, (uint4 *)workspace, (int)E, (int)M, (int)R,
+                                 (int)(K / 16));
     }
     if (e == cudaSuccess)
         e = few ? (e8 ? wf::grp::launch_pairs<true, 64>(p, sms, st) : wf::grp::launch_pairs<false, 64>(p, sms, st))
