@@ -574,3 +574,29 @@ def test_rms_norm_quant_overflowing_block():
     assert float(r.q[0, 130].float()) == 448.0
     e = _ops().rms_norm_quant(x, w, scale_fmt="ue8m0", scale_dtype=E8)
     assert bool(e.s[0, 0].float().isnan()) and bool(e.q[0, :128].float().isnan().all()) and not bool(e.s[0, 1].float().isnan())
+
+
+def test_small_outputs_are_tensors_of_their_own():
+    """Outputs that share an allocation do not overlap, have their own versions, and survive one another."""
+    ops = _ops()
+    g = _gen(43)
+    for T in (1, 5, 300, 4000):
+        x = torch.randn(T, 256, generator=g, device="cuda").bfloat16()
+        r = ops.rms_norm_quant(x, torch.ones(256, device="cuda"), residual=x, scale_fmt="ue8m0", scale_dtype=E8)
+        _check_norm(x, torch.ones(256, device="cuda"), x, r, True)
+        w, i = ops.route_topk(torch.randn(T, 64, generator=g, device="cuda"), 6)
+        d = ops.expert_dispatch(i, 64)
+        every = [r.q, r.s, r.y, r.h, w, i, *d]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in every)
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+        for t in every:
+            assert t.is_contiguous() and t.data_ptr() % 16 == 0 and not t._is_view() and t._version == 0
+        y, keep = r.y, r.y.clone()
+        r.q.view(torch.uint8).fill_(0)
+        assert y._version == 0
+        del r
+        other = [torch.full((T, 256), 7.0, device="cuda") for _ in range(8)]
+        assert torch.equal(y, keep) and len(other) == 8
+        i2 = i.clone()
+        i.add_(1)
+        assert torch.equal(i - 1, i2) and torch.equal(d[1], ops.expert_dispatch(i2, 64)[1])
