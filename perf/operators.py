@@ -178,7 +178,7 @@ def _own_route(c, st):
     from wanferenz_b200 import ops
 
     return ops.route_topk(st["logits"], c["k"], bias=st["bias"], score_func=c["score"], n_groups=c["groups"],
-                          topk_groups=c["keep"], group_score="top2", route_scale=1.5)
+                          topk_groups=c["keep"], route_scale=1.5)
 
 
 def _own_dispatch(c, st):
