@@ -161,6 +161,8 @@ def prepare(case, seed):
 def run(st):
     c = st["case"]
     if own:
+        if c["op"] == "route":  # names the group score: the operator's default without a bias is the largest
+            return _own_route_top2(c, st)
         return _OWN[c["op"]](c, st)
     return _PLAIN[c["op"]](c, st)
 
@@ -179,6 +181,13 @@ def _own_route(c, st):
 
     return ops.route_topk(st["logits"], c["k"], bias=st["bias"], score_func=c["score"], n_groups=c["groups"],
                           topk_groups=c["keep"], route_scale=1.5)
+
+
+def _own_route_top2(c, st):
+    from wanferenz_b200 import ops
+
+    return ops.route_topk(st["logits"], c["k"], bias=st["bias"], score_func=c["score"], n_groups=c["groups"],
+                          topk_groups=c["keep"], group_score="top2", route_scale=1.5)
 
 
 def _own_dispatch(c, st):
