@@ -425,3 +425,29 @@ def test_inference_mode_and_parameters():
         got = ops.rms_norm_quant(x, w)
     assert torch.equal(want.y, got.y) and torch.equal(want.s, got.s) and not want.y.requires_grad
     assert torch.equal(ops.rms_norm_quant(x, w).y, want.y)
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+@pytest.mark.parametrize("per", [3, 200])
+@pytest.mark.parametrize("K", [128, 512])
+def test_a_short_product_whose_wait_runs_out(kind, per, K):
+    """As few K steps as stages: the producer issues every copy without a wait of its own, and the CTA still leaves
+    only when they have landed.  The next call, in the same shared memory, is not affected."""
+    from wanferenz_b200 import _lib as L
+    ops = _ops()
+    g = _gen(16, per, K)
+    E, N = 4, 512
+    a, a_s, w, w_s = _operands(g, E * per, E, N, K, kind, kind)
+    off = _offsets([per] * E)
+    want = ops.grouped_fp8_gemm(a, a_s, w, w_s, off)
+    ops.grouped_read_error()
+    try:
+        L.check(L.load().wf_set_wait_limit(200), "wf_set_wait_limit")
+        ops.grouped_fp8_gemm(a, a_s, w, w_s, off)
+        with pytest.raises(L.WfError) as e:
+            ops.grouped_read_error()
+        assert e.value.code == L.WF_E_TIMEOUT
+    finally:
+        L.load().wf_set_wait_limit(0)
+    assert torch.equal(want, ops.grouped_fp8_gemm(a, a_s, w, w_s, off))
+    ops.grouped_read_error()

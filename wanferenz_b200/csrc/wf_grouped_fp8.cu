@@ -802,8 +802,9 @@ __global__ void __launch_bounds__(wide::THREADS, 1) k_grouped_f32_wide(const __g
                     }
                 }
             }
-            if (*abort)  // the copies issued must land before the CTA's memory goes
-                for (int u = max(0, gs - STAGES); u < gs; ++u) wf_wait(full + u % STAGES, (u / STAGES) & 1, &g_err);
+            // The copies issued must land before the CTA's memory goes, whoever gives up and whenever:
+            // a role whose wait runs out after this one has left its loop ends the CTA all the same.
+            for (int u = max(0, gs - STAGES); u < gs; ++u) wf_wait(full + u % STAGES, (u / STAGES) & 1, &g_err);
         } else if (warp == W_MMA) {
             const bool leader = elect_one();
             const uint64_t ad0 = smem_desc_sw128(base), bd0 = smem_desc_sw128(base + ABYTES);
