@@ -493,8 +493,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
                     if (++acc == NACC) { acc = 0; aphase ^= 1; }
                 }
             }
-            if (leader) commit2(fin, 1);  // TMEM and the peer's operands go only when every MMA is done
-            twait(fin, 0, abort, Bound{kWaitLimitCycles, 0});
+            if (leader) commit2(fin, 1);  // TMEM and the peer's operands go only when every MMA is done,
+            wf_wait(fin, 0, &g_err);      // also when the CTA gives up (twait would return at once)
         }
     } else if (warp < L::SCALE0) {
         // (no role)
@@ -829,8 +829,8 @@ __global__ void __launch_bounds__(wide::THREADS, 1) k_grouped_f32_wide(const __g
                     if (!acc) aphase ^= 1;
                 }
             }
-            if (leader) commit(fin);  // TMEM goes only when every MMA is done
-            twait(fin, 0, abort, Bound{kWaitLimitCycles, 0});
+            if (leader) commit(fin);  // TMEM goes only when every MMA is done,
+            wf_wait(fin, 0, &g_err);  // also when the CTA gives up (twait would return at once)
         }
     } else {
         // worker (q, half): the 32 tokens of TMEM lane quadrant q, 128 weight rows (one block of scales)
