@@ -2,8 +2,12 @@
 
 import glob
 import os
+import shutil
+
+import pytest
 
 from wanferenz_b200 import _build
+from wanferenz_b200 import _lib as L
 
 
 def test_every_source_and_header_of_the_library_is_watched():
@@ -12,3 +16,35 @@ def test_every_source_and_header_of_the_library_is_watched():
     device = {f for f in here if f.endswith((".cu", ".cuh", ".h"))}
     assert device and device <= set(_build.deps())
     assert set(glob.glob(os.path.join(_build.ROOT, "include", "*.h"))) <= set(_build.deps())
+
+
+@pytest.fixture
+def entry(tmp_path, monkeypatch):
+    """A Python entry module of the present source, torch and interpreter, in a folder of its own."""
+    L.load_ext()
+    for name in ("EXT", "EXT_KEY"):
+        shutil.copy(getattr(_build, name), tmp_path)
+        monkeypatch.setattr(_build, name, str(tmp_path / os.path.basename(getattr(_build, name))))
+    src = tmp_path / "wf_torch.cpp"
+    shutil.copy(_build.EXT_SRC, src)
+    monkeypatch.setattr(_build, "EXT_SRC", str(src))
+    monkeypatch.setattr(L, "_EXT", None)
+    return src
+
+
+def test_the_entry_module_in_place_is_current(entry):
+    assert _build.ext_current() and _build.build_ext() == _build.EXT
+
+
+@pytest.mark.parametrize("what", ["torch", "source", "key", "module"])
+def test_a_stale_entry_module_is_not_loaded(entry, monkeypatch, what):
+    """One built for another torch or from another source would be called with arguments that it does not have."""
+    if what == "torch":
+        monkeypatch.setattr("torch.__version__", "1.0.0")
+    elif what == "source":
+        entry.write_text(entry.read_text() + "// another\n")
+    else:
+        os.remove(_build.EXT if what == "module" else _build.EXT_KEY)
+    assert not _build.ext_current()
+    with pytest.raises(ImportError, match="entry module"):
+        L.load_ext(build_if_missing=False)

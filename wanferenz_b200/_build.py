@@ -10,6 +10,7 @@ statically links the CUDA runtime and is loaded with ctypes.  Beside it goes
 from __future__ import annotations
 
 import glob
+import hashlib
 import os
 import subprocess
 import sys
@@ -20,6 +21,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libwfb200.so")
 EXT = os.path.join(LIBDIR, "_wfb200_torch.so")
+EXT_KEY = EXT + ".key"
 EXT_SRC = os.path.join(CSRC, "wf_torch.cpp")
 
 NVCC_FLAGS = [
@@ -50,11 +52,33 @@ def ext_deps():
     return [EXT_SRC, os.path.join(ROOT, "include", "wfb200.h")]
 
 
-def up_to_date(target: str = LIB, of=None) -> bool:
-    if not os.path.exists(target):
+def up_to_date() -> bool:
+    if not os.path.exists(LIB):
         return False
-    t = os.path.getmtime(target)
-    return all(os.path.getmtime(p) <= t for p in (of or deps()))
+    t = os.path.getmtime(LIB)
+    return all(os.path.getmtime(p) <= t for p in deps())
+
+
+def ext_key() -> str:
+    """What the Python entry module is compiled from and against: its sources, torch, and the interpreter's ABI."""
+    import sysconfig
+
+    import torch
+
+    key = hashlib.sha256(f"{torch.__version__} {sysconfig.get_config_var('SOABI')}".encode())
+    for p in ext_deps():
+        with open(p, "rb") as f:
+            key.update(f.read())
+    return key.hexdigest()
+
+
+def ext_current() -> bool:
+    """Whether the module in place is of this source, torch and interpreter (by the key written beside it)."""
+    try:
+        with open(EXT_KEY) as f:
+            return os.path.exists(EXT) and f.read() == ext_key()
+    except FileNotFoundError:
+        return False
 
 
 def _run(cmd, target, verbose):
@@ -77,8 +101,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 def build_ext(force: bool = False, verbose: bool = False) -> str:
     """The Python entry module; links ``build()``'s library, which must exist."""
-    if not force and up_to_date(EXT, ext_deps()):
+    if not force and ext_current():
         return EXT
+    key = ext_key()
     import sysconfig
 
     import torch
@@ -92,6 +117,10 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     libs += ["-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
              "-L" + LIBDIR, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     _run([os.environ.get("CXX", "g++"), *flags, EXT_SRC, "-o", None, *libs], EXT, verbose)
+    tmp = EXT_KEY + f".tmp{os.getpid()}"
+    with open(tmp, "w") as f:
+        f.write(key)
+    os.replace(tmp, EXT_KEY)
     return EXT
 
 

@@ -148,14 +148,14 @@ def load_ext(build_if_missing: bool = True):
     global _EXT
     if _EXT is None:
         load(build_if_missing)
-        if not os.path.exists(_build.EXT):
+        import torch  # noqa: F401  (its libraries are the module's)
+
+        if not _build.ext_current():  # missing, or of another source, torch or Python: its calls would not fit
             if not build_if_missing:
-                raise ImportError(f"wanferenz_b200: entry module missing at {_build.EXT}; run "
+                raise ImportError(f"wanferenz_b200: no entry module for this torch and Python at {_build.EXT}; run "
                                   f"`python -m wanferenz_b200._build`")
             _build.build_ext()
         import importlib.util
-
-        import torch  # noqa: F401  (its libraries are the module's)
 
         spec = importlib.util.spec_from_file_location("_wfb200_torch", _build.EXT)
         ext = importlib.util.module_from_spec(spec)
