@@ -3,6 +3,7 @@
 import glob
 import os
 import shutil
+import sys
 
 import pytest
 
@@ -48,3 +49,25 @@ def test_a_stale_entry_module_is_not_loaded(entry, monkeypatch, what):
     assert not _build.ext_current()
     with pytest.raises(ImportError, match="entry module"):
         L.load_ext(build_if_missing=False)
+
+
+@pytest.mark.parametrize("lacks", ["compiler", "headers", "torch"])
+def test_the_library_builds_without_what_the_entry_module_needs(monkeypatch, capsys, lacks):
+    """A host of the C ABI has nvcc; the command builds the library there, says what is left out, and succeeds."""
+    monkeypatch.setattr(_build, "build", lambda force=False, verbose=False: "the library")
+    if lacks == "compiler":
+        monkeypatch.setenv("CXX", "/nonexistent/g++")
+    elif lacks == "headers":
+        monkeypatch.setattr("sysconfig.get_paths", lambda: {"include": "/nonexistent"})
+    else:
+        monkeypatch.setitem(sys.modules, "torch", None)
+    _build.main(["_build", "--force"])
+    seen = capsys.readouterr()
+    assert "the library" in seen.out and "not built" in seen.err
+
+
+def test_an_entry_module_that_does_not_compile_is_an_error(entry, monkeypatch):
+    monkeypatch.setattr(_build, "build", lambda force=False, verbose=False: "the library")
+    entry.write_text("#error no\n")
+    with pytest.raises(RuntimeError, match="failed"):
+        _build.main(["_build"])

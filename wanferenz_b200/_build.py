@@ -12,6 +12,7 @@ from __future__ import annotations
 import glob
 import hashlib
 import os
+import shutil
 import subprocess
 import sys
 
@@ -116,7 +117,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     libs = ["-L" + d for d in cpp_extension.library_paths(device_type="cuda")]
     libs += ["-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
              "-L" + LIBDIR, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
-    _run([os.environ.get("CXX", "g++"), *flags, EXT_SRC, "-o", None, *libs], EXT, verbose)
+    _run([cxx(), *flags, EXT_SRC, "-o", None, *libs], EXT, verbose)
     tmp = EXT_KEY + f".tmp{os.getpid()}"
     with open(tmp, "w") as f:
         f.write(key)
@@ -124,6 +125,36 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     return EXT
 
 
+def cxx() -> str:
+    return os.environ.get("CXX", "g++")
+
+
+def ext_lacks():
+    """What this machine lacks to compile the Python entry module (None: nothing)."""
+    import sysconfig
+
+    if shutil.which(cxx()) is None:
+        return f"a C++ compiler ({cxx()})"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers"
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return "torch"
+    return None
+
+
+def main(argv) -> None:
+    """The library always; the Python entry module where it can be compiled, since a host of the C ABI needs neither
+    torch nor Python's headers."""
+    force = "--force" in argv
+    print(build(force=force, verbose=True))
+    lacks = ext_lacks()
+    if lacks:
+        print(f"not built: {EXT}, the Python entry of the layer operators; this machine lacks {lacks}", file=sys.stderr)
+    else:
+        print(build_ext(force=force, verbose=True))
+
+
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose=True))
-    print(build_ext(force="--force" in sys.argv, verbose=True))
+    main(sys.argv)
