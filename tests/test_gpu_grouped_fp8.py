@@ -451,3 +451,104 @@ def test_a_short_product_whose_wait_runs_out(kind, per, K):
         L.load().wf_set_wait_limit(0)
     assert torch.equal(want, ops.grouped_fp8_gemm(a, a_s, w, w_s, off))
     ops.grouped_read_error()
+
+
+# Every path of the product by rows per expert: lists gathered in place, narrow tiles (lists packed first), wide tiles of
+# either kind of scales.  300 rows an expert are two wide tiles, so an entry may lie past columns 32, 64 and 128 of one.
+PATHS = [("gather", True, 12), ("narrow", True, 40), ("narrow", False, 40), ("wide", True, 300), ("wide", False, 300)]
+
+
+def _marked(t, at):
+    """`t` with the e4m3 rows `at` NaN, and with them zero."""
+    nan, zero = t.clone(), t.clone()
+    nan.view(torch.uint8)[at] = 0x7f
+    zero.view(torch.uint8)[at] = 0
+    return nan, zero
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+@pytest.mark.parametrize("path,listed,per", PATHS)
+@pytest.mark.parametrize("N,K", [(264, 384), (128, 1024)])
+def test_gaps_and_bad_rows_on_every_path(kind, path, listed, per, N, K):
+    """Rows of no expert stay as they were, NaN rows right behind an expert's last row do not reach it, and entries
+    outside [0, M) give zeros wherever in a tile they stand, though row 0 of a is NaN."""
+    g = _gen(17, path, listed, N)
+    E, R = 3, 3 * per
+    M = 50 if listed else R
+    a, a_s, w, w_s = _operands(g, M, E, N, K, kind, kind)
+    ends = [3, per - 3, per + 2, 2 * per + 5, R - 4]
+    off = torch.tensor([ends[0], ends[1], 2 * per + 5, ends[4]], device="cuda").int()  # rows before, none between, behind
+    if listed:
+        a, clean = _marked(a, [0, M - 1])
+        rows = torch.randint(1, M - 1, (R,), generator=g, device="cuda").int()
+        rows[:ends[0]] = 0
+        rows[ends[4]:] = M - 1
+        bad = [p for p in (3, 3 + 33, 3 + 66, 3 + 130, per - 4, per + 40, 2 * per + 4, R - 5) if 3 <= p < R - 4]
+        for j, p in enumerate(bad):
+            rows[p] = (-1, M, 2 ** 31 - 1, -2 ** 31)[j % 4]
+    else:
+        a, clean = _marked(a, list(range(ends[0])) + list(range(ends[4], R)))
+        rows, bad = None, []
+    out = torch.full((R, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    _ops().grouped_fp8_gemm(a, a_s, w, w_s, off, rows=rows, out=out)
+    _check(out, clean, a_s, w, w_s, off, rows)
+    assert bool((out[:ends[0]] == 7).all()) and bool((out[ends[4]:] == 7).all())
+    assert not bad or not out[bad].any()
+    # an expert without rows between two with rows, its neighbours' rows NaN to one another
+    off = torch.tensor([0, ends[1], ends[1], ends[2]], device="cuda").int()
+    out.fill_(7.0)
+    _ops().grouped_fp8_gemm(clean, a_s, w, w_s, off, rows=rows, out=out)
+    _check(out, clean, a_s, w, w_s, off, rows)
+    assert bool((out[ends[2]:] == 7).all())
+    _ops().grouped_read_error()
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+@pytest.mark.parametrize("path,listed,per", PATHS)
+def test_clamped_and_falling_offsets_on_every_path(kind, path, listed, per):
+    """Offsets outside [0, R] are clamped to it; an expert whose end lies before its start has no rows."""
+    g = _gen(18, path, listed)
+    E, R, N, K = 3, 3 * per, 136, 256
+    M = 40 if listed else R
+    a, a_s, w, w_s = _operands(g, M, E, N, K, kind, kind)
+    rows = torch.randint(0, M, (R,), generator=g, device="cuda").int() if listed else None
+    for off in ([-2 ** 31, per, R - 1, 2 ** 31 - 1], [2 * per, per, 2 * per + 1, per + 1], [R, R, R + 5, 0], [R + 1, -1, 1, 0]):
+        off = torch.tensor(off, device="cuda").int()
+        out = torch.full((R, N), 7.0, dtype=torch.bfloat16, device="cuda")
+        _ops().grouped_fp8_gemm(a, a_s, w, w_s, off, rows=rows, out=out)
+        inside = off.clamp(0, R)
+        _check(out, a, a_s, w, w_s, inside, rows)
+        owned = torch.zeros(R, dtype=torch.bool, device="cuda")
+        lo, hi = inside[:-1].tolist(), inside[1:].tolist()
+        for x, y in zip(lo, hi):
+            owned[x:max(x, y)] = True
+        assert bool((out[~owned] == 7).all())
+    _ops().grouped_read_error()
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+@pytest.mark.parametrize("path,listed,per", PATHS)
+def test_nan_stays_in_its_row_or_block_on_every_path(kind, path, listed, per):
+    g = _gen(19, path, listed)
+    E, R, N, K = 2, 2 * per, 264, 512
+    a, a_s, w, w_s = _operands(g, R, E, N, K, kind, kind)
+    off = _offsets([per, per])
+    rows = torch.randperm(R, generator=g, device="cuda").int() if listed else None
+    named = rows.long() if listed else torch.arange(R, device="cuda")
+    at = [1, per // 2, per - 1, per + 2]  # rows of the product
+    a.view(torch.uint8)[named[at[0]], 130] = 0x7f
+    a.view(torch.uint8)[named[at[1]], 511] = 0xff
+    a_s[named[at[2]], 2] = float("nan")
+    a_s[named[at[3]], 0] = float("nan")
+    if kind == E8:
+        w_s.view(torch.uint8)[1, 1, 3] = 255
+    else:
+        w_s[1, 1, 3] = float("nan")
+    w.view(torch.uint8)[0, 263, 5] = 0x7f
+    out = _ops().grouped_fp8_gemm(a, a_s, w, w_s, off, rows=rows)
+    want = torch.zeros(R, N, dtype=torch.bool, device="cuda")
+    want[at] = True
+    want[per:, 128:256] = True
+    want[:per, 263] = True
+    assert torch.equal(out.isnan(), want)
+    _ops().grouped_read_error()
