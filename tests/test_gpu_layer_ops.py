@@ -600,3 +600,32 @@ def test_small_outputs_are_tensors_of_their_own():
         i2 = i.clone()
         i.add_(1)
         assert torch.equal(i - 1, i2) and torch.equal(d[1], ops.expert_dispatch(i2, 64)[1])
+
+
+def test_rms_norm_quant_divides_like_a_division():
+    """q is what e4m3 of the float32 quotient n / s gives, on random values and next to every e4m3 midpoint.
+
+    A row of ones with eps 0 has the norm 1, so n is the weight.  The one dividend that differs by a step, a power of two
+    over a scale whose significand is all ones, does not occur: no scale here has that significand."""
+    mids = [(2 * m + 1) * 2.0 ** -10 for m in range(8)] + [(2 * m + 17) * 2.0 ** (e - 4) for e in range(-6, 9) for m in range(8)]
+    mids = torch.tensor([m for m in mids if m < 448], dtype=torch.float64, device="cuda")
+    g = _gen(5)
+    D = 16384
+    x = torch.ones(1, D, dtype=torch.bfloat16, device="cuda")
+    for k in range(48):
+        top = torch.rand(D // 128, 1, generator=g, device="cuda") + 1
+        top = top * torch.exp2(torch.randint(-9, 12, top.shape, generator=g, device="cuda").float())
+        s = top * torch.tensor(1.0 / 448, device="cuda")
+        assert not bool(((s.view(torch.int32) & 0x7fffff) == 0x7fffff).any())
+        if k % 3 == 0:
+            n = top * torch.rand(D // 128, 128, generator=g, device="cuda")
+        else:  # within three float32 steps of a midpoint times the scale
+            m = mids[torch.randint(0, mids.numel(), (D // 128, 128), generator=g, device="cuda")]
+            n = (m * s.double()).float()
+            n = (n.view(torch.int32) + torch.randint(-3, 4, n.shape, generator=g, device="cuda").int()).view(torch.float32)
+            n = torch.minimum(n, top)
+        n = torch.where(torch.rand(n.shape, generator=g, device="cuda") < 0.5, n, -n)
+        n[:, 7] = top[:, 0]
+        r = _ops().rms_norm_quant(x, n.reshape(-1), 0.0)
+        assert torch.equal(r.s[0], s[:, 0])
+        assert torch.equal(r.q[0].float(), (n / s).clamp(-448, 448).to(torch.float8_e4m3fn).float().reshape(-1))

@@ -201,8 +201,12 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
                 byte = s < CUDART_INF_F ? (b + 0x7fffffu) >> 23 : 0xffu;
                 s = byte < 0xffu ? __uint_as_float(byte << 23) : CUDART_NAN_F;
             }
-            // n / s: exact by the reciprocal of a power of two (below 2^120, as n is finite); else the
-            // product with the rounded reciprocal is put right by its remainder (0 for an infinite s)
+            // n / s: exact by the reciprocal of a power of two (below 2^120, as n is finite).  Else
+            // Markstein's division (IBM J. Res. Dev. 34, 1990): the product with the rounded reciprocal
+            // plus the reciprocal times the remainder (0 for an infinite s) is the rounded quotient,
+            // but for a significand of s that is all ones: a power of two over it comes out a step low.
+            // That moves one q, n / s next above 2^-10 (to 0, not 2^-9); every other significand of s,
+            // with the dividends nearest every e4m3 midpoint, was tried on the CPU.
             const float inv = !p.ue8m0 ? __frcp_rn(s) : byte < 0xffu ? __uint_as_float((254u - byte) << 23) : CUDART_NAN_F;
             float2 u[4];
 #pragma unroll
