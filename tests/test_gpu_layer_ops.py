@@ -629,3 +629,23 @@ def test_rms_norm_quant_divides_like_a_division():
         r = _ops().rms_norm_quant(x, n.reshape(-1), 0.0)
         assert torch.equal(r.s[0], s[:, 0])
         assert torch.equal(r.q[0].float(), (n / s).clamp(-448, 448).to(torch.float8_e4m3fn).float().reshape(-1))
+
+
+def test_outputs_have_memory_of_their_own():
+    """An output may be grown, shrunk to nothing or saved as any tensor; the call's other outputs stay as they are."""
+    ops = _ops()
+    g = _gen(44)
+    x = torch.randn(5, 256, generator=g, device="cuda").bfloat16()
+    r = ops.rms_norm_quant(x, torch.ones(256, device="cuda"), residual=x)
+    w, i = ops.route_topk(torch.randn(5, 64, generator=g, device="cuda"), 6)
+    d = ops.expert_dispatch(i, 64)
+    every = [r.q, r.s, r.y, r.h, w, i, *d]
+    assert len({t.untyped_storage().data_ptr() for t in every}) == len(every)
+    assert all(t.untyped_storage().nbytes() == t.numel() * t.element_size() and t.storage_offset() == 0 for t in every)
+    keep = [t.clone() for t in every]
+    w.resize_(64, 6).fill_(-5)
+    d[0].resize_(512).fill_(-5)
+    r.s.untyped_storage().resize_(0)
+    for t, k in zip(every, keep):
+        if t is not w and t is not d[0] and t is not r.s:
+            assert torch.equal(t.view(torch.uint8), k.view(torch.uint8))

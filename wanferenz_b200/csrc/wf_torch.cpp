@@ -81,54 +81,12 @@ bool truth(PyObject *o) {
     return v != 0;
 }
 
+// An output: each has an allocation of its own, so that a caller may resize, free or save one and leave
+// the others alone.  (One allocation for all of a call's took 0.4 to 0.9 us less at a few tokens, and
+// growing an output in place then ran into its neighbour.)
 at::Tensor empty(at::IntArrayRef s, ScalarType type, const at::Device &dev) {
     return at::detail::empty_cuda(s, type, dev, std::nullopt);
 }
-
-// Outputs of one call that live and die together.  Small ones share one allocation, since at a few
-// tokens an allocation and its release cost the host as much as a launch; from 1 MiB on each has its
-// own, so that keeping one does not keep the others' memory.  Each part starts on 256 bytes, as an
-// allocation of its own would on 512, and is a tensor with its own version, not a view.  Host time of a
-// call, own allocations -> one: norm of 1 row 6.8 -> 5.8 us, routing of 16 tokens 4.7 -> 4.1 us,
-// dispatch of 64 x 6 slots 5.5 -> 4.6 us.
-class Outputs {
-  public:
-    explicit Outputs(const at::Device &dev) : dev_(dev) {}
-    void add(at::Tensor *out, at::IntArrayRef sizes, ScalarType type) {
-        size_t bytes = c10::elementSize(type);
-        for (int64_t n : sizes) bytes *= (size_t)n;
-        parts_[count_++] = {out, c10::DimVector(sizes), type, total_};
-        total_ += (bytes + 255) & ~size_t(255);
-    }
-    void make() {
-        if (count_ < 2 || total_ > size_t(1) << 20) {
-            for (int i = 0; i < count_; ++i) *parts_[i].out = empty(parts_[i].sizes, parts_[i].type, dev_);
-            return;
-        }
-        const at::Tensor block = empty({(int64_t)total_}, at::kByte, dev_);
-        for (int i = 0; i < count_; ++i) {
-            const Part &p = parts_[i];
-            at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()),
-                                                                    c10::DispatchKeySet(c10::DispatchKey::CUDA),
-                                                                    c10::scalarTypeToTypeMeta(p.type));
-            t.unsafeGetTensorImpl()->set_storage_offset((int64_t)(p.at / c10::elementSize(p.type)));
-            t.unsafeGetTensorImpl()->set_sizes_contiguous(p.sizes);
-            *p.out = std::move(t);
-        }
-    }
-
-  private:
-    struct Part {
-        at::Tensor *out;
-        c10::DimVector sizes;
-        ScalarType type;
-        size_t at;
-    };
-    at::Device dev_;
-    Part parts_[4];
-    int count_ = 0;
-    size_t total_ = 0;
-};
 
 void *ptr(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 int kind(const at::Tensor &t) { return t.scalar_type() == at::kFloat ? WF_SCALE_F32 : WF_SCALE_E8M0; }
@@ -202,12 +160,8 @@ WF_ENTRY(rms_norm_quant, 7) {
     if (st != at::kFloat && !ue8m0) raise(PyExc_ValueError, "e8m0 scales need scale_fmt (power-of-two rounding)");
     c10::DimVector ss(x.sizes());
     ss.back() = d / 128;
-    at::Tensor q, s;
-    Outputs outs(dev);  // (h, the residual stream, outlives them)
-    outs.add(&q, x.sizes(), at::kFloat8_e4m3fn);
-    outs.add(&s, ss, st);
-    if (truth(a[4])) outs.add(&y, x.sizes(), at::kBFloat16);
-    outs.make();
+    const at::Tensor q = empty(x.sizes(), at::kFloat8_e4m3fn, dev), s = empty(ss, st, dev);
+    if (truth(a[4])) y = empty(x.sizes(), at::kBFloat16, dev);
     if (x.numel())
         run(dev, "wf_rms_norm_quant", [&](void *stream) {
             return wf_rms_norm_quant(ptr(x), ptr(res), ptr(w), w.scalar_type() == at::kBFloat16, x.numel() / d, d, (float)eps,
@@ -237,11 +191,7 @@ WF_ENTRY(route_topk, 9) {
         raise(PyExc_ValueError, "topk %lld must be in 1..min(16, experts of topk_groups groups)", k);
     const bool top2 = truth(a[6]), renorm = truth(a[7]);
     const double scale = number(a[8]);
-    at::Tensor w, i;
-    Outputs outs(dev);
-    outs.add(&w, {t, k}, at::kFloat);
-    outs.add(&i, {t, k}, at::kLong);
-    outs.make();
+    const at::Tensor w = empty({t, k}, at::kFloat, dev), i = empty({t, k}, at::kLong, dev);
     if (t)
         run(dev, "wf_route_topk", [&](void *stream) {
             return wf_route_topk(ptr(l), l.scalar_type() == at::kBFloat16, (const float *)ptr(bias), t, (int32_t)e, (int32_t)k,
@@ -262,12 +212,8 @@ WF_ENTRY(expert_dispatch, 3) {
         raise(PyExc_ValueError, "indices [%lld, %lld] over %lld experts: k in 1..16, 1 to 512 experts, at most 2^30 pairs",
               (long long)t, (long long)k, n);
     if (base < 0 || base > 0x7fffffff - 512) raise(PyExc_ValueError, "expert_offset %lld out of range", base);
-    at::Tensor offsets, tokens, slots;
-    Outputs outs(dev);
-    outs.add(&offsets, {n + 1}, at::kInt);
-    outs.add(&tokens, {t * k}, at::kInt);
-    outs.add(&slots, {t, k}, at::kInt);
-    outs.make();
+    const at::Tensor offsets = empty({n + 1}, at::kInt, dev), tokens = empty({t * k}, at::kInt, dev);
+    const at::Tensor slots = empty({t, k}, at::kInt, dev);
     if (!t) return pack({offsets.zero_(), tokens, slots});
     const size_t need = wf_expert_dispatch_workspace_bytes(t, (int32_t)k, (int32_t)n);
     at::Tensor ws;
