@@ -362,7 +362,8 @@ int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32
  * tokens), out [R, N] bf16.  Sums are in 32 bits.  offsets are clamped to
  * [0, R], rows of out that belong to no expert are not written, and a row list
  * entry outside [0, M) gives a row of zeros.  N a multiple of 8, K of 128, E in
- * 1..512; a, w and out 16-byte aligned.  Device waits are bounded; one that runs
+ * 1..512; a, w and out 16-byte aligned; out and the workspace apart from one another
+ * and from every input.  Device waits are bounded; one that runs
  * out ends the call early and shows in wf_grouped_read_error. */
 int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, const void *w,
                         const void *w_s, int32_t w_scale_kind, const int32_t *offsets,

@@ -107,3 +107,22 @@ def _grouped(a=P, a_s=P, ak=F32, w=P, w_s=P, wk=F32, off=P, rows=P, M=8, R=12, E
     (dict(out=ctypes.c_void_p(4104)), L.WF_E_ARG), (dict(a_s=ODD), L.WF_E_ARG), (dict(rows=ODD), L.WF_E_ARG)])
 def test_grouped_fp8_gemm_refuses(kw, code):
     assert _grouped(**kw) == code
+
+
+AT = {"a": 1 << 40, "a_s": 2 << 40, "w": 3 << 40, "w_s": 4 << 40, "off": 5 << 40, "rows": 6 << 40, "ws": 7 << 40}
+
+
+@pytest.mark.parametrize("name,size", [("a", 8 * 256), ("a_s", 8 * 2 * 4), ("w", 4 * 256 * 256), ("w_s", 4 * 2 * 2 * 4),
+                                       ("off", 5 * 4), ("rows", 1024 * 4), ("ws", 1024 * 256)])
+@pytest.mark.parametrize("side", ["front", "end"])
+def test_grouped_fp8_gemm_refuses_an_output_over_an_input(name, size, side):
+    """Other rows' results would be read as inputs; a workspace over an input is the same."""
+    ptr = {k: ctypes.c_void_p(v) for k, v in AT.items()}
+    out = AT[name] - 1024 * 256 * 2 + 16 if side == "front" else AT[name] + (size - 1) // 16 * 16
+    kw = dict(R=1024, n=1024 * 256, **ptr)
+    assert _grouped(out=ctypes.c_void_p(out), **kw) == L.WF_E_ARG
+    assert b"overlap" in L.load().wf_last_error()
+    if name != "ws":
+        kw["ws"] = ctypes.c_void_p(AT[name] - 1024 * 256 + 16 if side == "front" else AT[name] + (size - 1) // 16 * 16)
+        assert _grouped(out=ctypes.c_void_p(8 << 40), **kw) == L.WF_E_ARG
+        assert b"overlap" in L.load().wf_last_error()

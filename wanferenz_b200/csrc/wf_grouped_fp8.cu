@@ -936,6 +936,16 @@ __global__ void __launch_bounds__(32 * PACK_WARPS) k_pack_rows(const uint4 *a, c
     }
 }
 
+// Memory of a call: what it writes must lie apart from what its CTAs read at other times.
+struct Span {
+    const void *at;
+    int64_t bytes;
+    bool meets(const Span &o) const {
+        const uintptr_t x = (uintptr_t)at, y = (uintptr_t)o.at;
+        return bytes > 0 && o.bytes > 0 && x < y + (uintptr_t)o.bytes && y < x + (uintptr_t)bytes;
+    }
+};
+
 int tensor_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t K, uint32_t box_rows) {
     host::EncodeTiledFn enc = host::encode_fn();
     if (!enc) return host::fail(WF_E_CUDA, "cuTensorMapEncodeTiled unavailable");
@@ -1004,6 +1014,13 @@ int wf_grouped_fp8_gemm(const void *a, const void *a_s, int32_t a_scale_kind, co
         if (!workspace || workspace_bytes < (size_t)R * K) return fail(WF_E_ARG, "workspace too small (see wf_grouped_fp8_workspace_bytes)");
         if ((uintptr_t)workspace % 16) return fail(WF_E_ARG, "workspace must be 16-byte aligned");
     }
+    const int64_t nks = K / 128, a_sb = a_scale_kind == WF_SCALE_F32 ? 4 : 1, w_sb = w_scale_kind == WF_SCALE_F32 ? 4 : 1;
+    const wf::grp::Span in[] = {{a, M * K},      {a_s, M * nks * a_sb},    {w, E * N * K}, {w_s, E * ((N + 127) / 128) * nks * w_sb},
+                                {offsets, (E + 1) * 4}, {rows, rows ? R * 4 : 0}};
+    const wf::grp::Span y = {out, R * N * 2}, ws = {workspace, pack ? R * K : 0};
+    for (const wf::grp::Span &x : in)
+        if (x.meets(y) || x.meets(ws)) return fail(WF_E_ARG, "out or the workspace overlaps an input");
+    if (y.meets(ws)) return fail(WF_E_ARG, "out overlaps the workspace");
     p.gather = rows && !pack;
     int rc = wf::grp::tensor_map(&p.tmW, w, (uint64_t)E * N, K, 128);
     if (p.gather) {

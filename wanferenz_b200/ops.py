@@ -250,7 +250,7 @@ def grouped_fp8_gemm(a, a_s, w, w_s, offsets, *, rows=None, out=None):
     K/128]``, scales f32 or e8m0 (as ``act_quant`` and ``rms_norm_quant`` give them); ``offsets
     [E + 1]`` and ``rows [R]`` int32 on the device, as ``expert_dispatch`` gives them (its
     ``tokens`` gather a token's row for each of its experts, so no permuted copy is made).
-    Returns bf16 ``[R, N]`` (``out`` when given); rows behind ``offsets[E]`` are not written.  An
+    Returns bf16 ``[R, N]`` (``out`` when given, which must not overlap an input); rows behind ``offsets[E]`` are not written.  An
     entry of ``rows`` outside ``[0, M)`` gives a row of zeros.  N a multiple of 8, K of 128.
     """
     return _ext().grouped_fp8_gemm(a, a_s, w, w_s, offsets, rows, out)
