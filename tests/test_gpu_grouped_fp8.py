@@ -552,3 +552,20 @@ def test_nan_stays_in_its_row_or_block_on_every_path(kind, path, listed, per):
     want[:per, 263] = True
     assert torch.equal(out.isnan(), want)
     _ops().grouped_read_error()
+
+
+def test_a_given_output_counts_as_changed():
+    """A graph that holds `out` from before the call says so in its backward pass, as for any write in place."""
+    g = _gen(20)
+    a, a_s, w, w_s = _operands(g, 10, 2, 128, 128, E8, E8)
+    out = torch.zeros(10, 128, dtype=torch.bfloat16, device="cuda")
+    factor = torch.ones(10, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    held = (out * factor).sum()
+    _ops().grouped_fp8_gemm(a, a_s, w, w_s, _offsets([4, 6]), out=out)
+    assert out._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        held.backward()
+    with torch.inference_mode():
+        inner = torch.zeros_like(out)
+        assert _ops().grouped_fp8_gemm(a, a_s, w, w_s, _offsets([4, 6]), out=inner) is inner
+    assert torch.equal(_ops().grouped_fp8_gemm(a, a_s, w, w_s, _offsets([4, 6]), out=inner), out)

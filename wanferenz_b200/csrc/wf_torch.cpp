@@ -261,6 +261,8 @@ WF_ENTRY(grouped_fp8_gemm, 7) {
     }
     if (r) {
         if (!m) raise(PyExc_ValueError, "a has no rows to take");
+        // a graph that saved the caller's out must see that its values change
+        if (a[6] != Py_None && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
         at::Tensor ws;
         const size_t need = wf_grouped_fp8_workspace_bytes(rows.defined(), r, (int32_t)e, k);
         if (need) ws = empty({(int64_t)need}, at::kByte, dev);
