@@ -649,3 +649,19 @@ def test_outputs_have_memory_of_their_own():
     for t, k in zip(every, keep):
         if t is not w and t is not d[0] and t is not r.s:
             assert torch.equal(t.view(torch.uint8), k.view(torch.uint8))
+
+
+def test_lazily_negated_inputs():
+    """The imaginary part of a conjugate is a float32 view whose memory holds the negatives."""
+    ops = _ops()
+    g = _gen(45)
+    z = torch.randn(1, 1, generator=g, device="cuda") + 1j * (torch.rand(1, 1, generator=g, device="cuda") + 1)
+    rows = torch.randn(1, 256, generator=g, device="cuda").bfloat16()
+    slots = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    w = z.conj().imag
+    assert w.is_neg() and w.is_contiguous()
+    got = ops.expert_combine(rows, slots, weights=w, out_dtype=torch.float32)
+    assert torch.equal(got, -z.imag.clone() * rows.float())
+    logits = torch.randn(3, 64, generator=g, device="cuda")
+    for a, b in zip(ops.route_topk(torch._neg_view(logits), 6), ops.route_topk(-logits, 6)):
+        assert torch.equal(a, b)

@@ -50,6 +50,7 @@ at::Tensor tensor(PyObject *o, const char *name, std::initializer_list<ScalarTyp
     if (!ok) raise(PyExc_TypeError, "%s has dtype %s, expected %s", name, c10::toString(t.scalar_type()), types_text);
     if (dev && t.device() != *dev)
         raise(PyExc_ValueError, "%s is on %s, expected %s", name, t.device().str().c_str(), dev->str().c_str());
+    if (t.is_neg()) return t.resolve_neg().contiguous();  // its memory holds the values' negatives
     if (!t.is_contiguous()) return t.contiguous();
     return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t;
 }
