@@ -562,7 +562,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
             for (int u = max(0, sg - 2); ok && u < sg; ++u) ok = twait(sf_empty + (u & 1), (u / 2) & 1, abort, p.limit);
         } else {
             // token scale x weight scale of each K step into shared memory
-                float *sa = reinterpret_cast<float *>(base + L::OFF_S);
+            float *sa = reinterpret_cast<float *>(base + L::OFF_S);
             const int i = threadIdx.x - 32 * L::SCALE0;  // this thread: tokens i, i + 64, ...
             int sg = 0;
             bool ok = true;

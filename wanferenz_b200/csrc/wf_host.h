@@ -44,10 +44,12 @@ inline cudaError_t allow_smem(const void *kernel, int which, size_t bytes, std::
 
 // Launches `kernel` so that it may start while the kernel before it on the stream drains
 // (programmatic dependent launch).  Every CTA of `kernel` executes griddepcontrol.wait before it
-// touches global memory, so the order of the stream holds for what it reads and writes.  Only the
+// touches global memory, so the order of the stream holds for what it reads and writes.  One
+// exception: k_dispatch_place behind k_dispatch_count reads the indices before its wait.  Only the
 // first kernel of an operator's two lets the next start early (griddepcontrol.launch_dependents),
-// behind its own wait, when all before it is done: the framework's products read their weights
-// ahead of their wait, so no kernel whose output a caller may pass on does.
+// and it must do so behind its own wait, when all before it is done: that exception rests on it.
+// The framework's products read their weights ahead of their wait, so no kernel whose output a
+// caller may pass on lets the next start early.
 template <class... P, class... A>
 cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};

@@ -655,7 +655,7 @@ __device__ __forceinline__ void disp_load(const DispArgs &p, int i0, int hi, int
 __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_count(const __grid_constant__ DispArgs p) {
     __shared__ int cnt[DISP_MAX_E];
     pdl_wait();
-    pdl_launch_dependents();
+    pdl_launch_dependents();  // behind the wait: k_dispatch_place reads the indices without one of its own
     const int warp = threadIdx.x >> 5;
     const int lo = min(p.pairs, (blockIdx.x * DISP_WARPS + warp) * p.run), hi = min(p.pairs, lo + p.run);
     int e[DISP_LANE];
