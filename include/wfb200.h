@@ -326,7 +326,7 @@ int wf_rms_norm_quant(const void *x, const void *residual, const void *weight, i
  * groups, which the reference's Gate does not have.  s = score(logit), sel =
  * s + bias (bias [E] f32 or NULL); of n_groups groups of E / n_groups
  * neighbouring experts the topk_groups with the largest value stay (the sum of
- * the group's two largest sel with group_top2, else its largest); the topk
+ * the group's two largest sel with group_top2, or the one that is not -infinity, else its largest); the topk
  * largest sel among them are chosen, in descending order, ties to the lower
  * index.  out_weights [T, topk] f32 = s (divided by their sum with renorm) *
  * route_scale; out_indices [T, topk] int64.  Scores are computed in 64 bits.  A
@@ -359,7 +359,8 @@ int wf_expert_dispatch(const void *indices, int32_t indices_64, int64_t T, int32
  * with i = rows[r], or r without a row list.  a [M, K] e4m3, a_s [M, K/128],
  * w [E, N, K] e4m3, w_s [E, ceil(N/128), K/128], scales f32 or e8m0; offsets
  * [E + 1] and rows [R] int32 on the device (wf_expert_dispatch's offsets and
- * tokens), out [R, N] bf16.  Sums are in 32 bits.  offsets are clamped to
+ * tokens), out [R, N] bf16.  Sums are in 32 bits, and so is the product of two f32 scales (it must
+ * neither overflow nor fall below the normal range).  offsets are clamped to
  * [0, R], rows of out that belong to no expert are not written, and a row list
  * entry outside [0, M) gives a row of zeros.  N a multiple of 8, K of 128, E in
  * 1..512; a, w and out 16-byte aligned; out and the workspace apart from one another

@@ -569,3 +569,28 @@ def test_a_given_output_counts_as_changed():
         inner = torch.zeros_like(out)
         assert _ops().grouped_fp8_gemm(a, a_s, w, w_s, _offsets([4, 6]), out=inner) is inner
     assert torch.equal(_ops().grouped_fp8_gemm(a, a_s, w, w_s, _offsets([4, 6]), out=inner), out)
+
+
+@pytest.mark.parametrize("kind", [torch.float32, E8])
+def test_a_bounded_list_of_local_rows(kind):
+    """A rank's experts with the list of all pairs, and with its first rows alone (narrower tiles): the same values up
+    to the order of the sums, through to the rank's partial sums."""
+    ops = _ops()
+    g = _gen(21)
+    T, k, ranks, E, N, K = 256, 4, 8, 4, 256, 512
+    idx = torch.rand(T, ranks * E, generator=g, device="cuda").topk(k, dim=-1).indices
+    a, a_s, w, w_s = _operands(g, T, E, N, K, kind, kind)
+    off, tok, slots = ops.expert_dispatch(idx, E, expert_offset=2 * E)
+    n = int(off[-1])
+    bound = n + 5
+    assert bound < 48 * E < T * k
+    whole = ops.grouped_fp8_gemm(a, a_s, w, w_s, off, rows=tok)
+    part = ops.grouped_fp8_gemm(a, a_s, w, w_s, off, rows=tok[:bound])
+    assert part.shape == (bound, N)
+    _check(whole, a, a_s, w, w_s, off, tok)
+    _check(part, a, a_s, w, w_s, off, tok)
+    y = ops.expert_combine(part, slots, out_dtype=torch.float32).double()
+    local = slots.clamp(min=0).long()
+    want = (part[local].double() * (slots >= 0)[..., None]).sum(1)
+    mag = (part[local].double().abs() * (slots >= 0)[..., None]).sum(1)
+    assert bool(((y - want).abs() <= mag * (k + 1) * 2.0 ** -24).all())

@@ -20,7 +20,9 @@ way from the residual stream through the experts' products and back:
 * ``expert_combine(rows, slots, weights)``      the experts' rows back in token order
 
 These run on their tensors' device (which need not be the current one) and on its
-current stream, keep nothing between calls, and have no gradients.
+current stream, keep nothing between calls, and have no gradients.  An input that is
+not contiguous, or starts off a 16-byte boundary, is copied first, on every call: keep
+weights contiguous.
 
 All tensors must be CUDA tensors; there is no CPU path.  Outputs are bf16,
 as the reference's are under the model's bf16 default dtype.
@@ -205,8 +207,8 @@ def route_topk(logits, topk, *, bias=None, score_func="sigmoid", n_groups=1, top
     ``Gate.forward`` (architecture.py:699-718) for any number of tokens, with a choice limited
     to groups: ``s = score(logit)``, ``sel = s + bias``; of ``n_groups`` groups of neighbouring
     experts the ``topk_groups`` with the largest value stay (``group_score`` "top2": the sum of
-    the group's two largest ``sel``, "max": its largest; by default "top2" with a bias and "max"
-    without); the ``topk`` largest ``sel`` among them are chosen, in descending order, equal ones
+    the group's two largest ``sel``, or the one that is not masked, "max": its largest; by default
+    "top2" with a bias and "max" without); the ``topk`` largest ``sel`` among them are chosen, in descending order, equal ones
     by ascending index.  ``weights = s / sum(s) * route_scale``, without the division for
     ``renormalize=False`` (the default for softmax, as in Gate).
 
@@ -250,8 +252,15 @@ def grouped_fp8_gemm(a, a_s, w, w_s, offsets, *, rows=None, out=None):
     K/128]``, scales f32 or e8m0 (as ``act_quant`` and ``rms_norm_quant`` give them); ``offsets
     [E + 1]`` and ``rows [R]`` int32 on the device, as ``expert_dispatch`` gives them (its
     ``tokens`` gather a token's row for each of its experts, so no permuted copy is made).
-    Returns bf16 ``[R, N]`` (``out`` when given, which must not overlap an input); rows behind ``offsets[E]`` are not written.  An
-    entry of ``rows`` outside ``[0, M)`` gives a row of zeros.  N a multiple of 8, K of 128.
+    Returns bf16 ``[R, N]`` (``out`` when given, which must not overlap an input); rows behind
+    ``offsets[E]`` are not written.  An entry of ``rows`` outside ``[0, M)`` gives a row of zeros.
+    N a multiple of 8, K of 128.  With f32 scales the product of a row's and a block's scale is a
+    32-bit value, and must not overflow or fall below the normal range.
+
+    Tiles, workspace and output go by ``R``, all rows of the list.  With the experts split over
+    ranks most of ``expert_dispatch``'s list belongs to no local expert: the result is right, the
+    tiles are wider than the local rows need.  A program that knows a bound of at least
+    ``offsets[E]`` passes ``rows=tokens[:bound]``.
     """
     return _ext().grouped_fp8_gemm(a, a_s, w, w_s, offsets, rows, out)
 
