@@ -21,10 +21,13 @@
 // lanes read the same ones or not: 131 KB a K step, as many cycles as the whole product.)
 //
 // Measured on a B200.  Few rows per expert, bound by the weights' stream (5.5 TB/s while it
-// runs): 96 rows over 64 experts of 2048 x 2048, e8m0, 41 us (floor 32); 1536 rows over 64 of
-// 2048 x 1024, f32, 33.7 us (21.7).  Many, bound by the tensor cores and by power: one expert of
-// 16384 rows, 4096 x 4096, e8m0, 3.05 PFLOP/s in a burst, 2.4 sustained under the 1 kW cap; 16386
-// rows over 32 of these experts 256 us in a burst (174), 336 sustained; with f32 scales 390.
+// runs): 96 rows over 64 experts of 2048 x 2048, e8m0, 40 us (floor 32); 1536 rows over 64 of
+// 2048 x 1024, f32, 35.4 us (21.7).  Many: one expert of 16384 rows, 4096 x 4096, e8m0, 2.7 to 2.8
+// PFLOP/s in a call by itself, 2.3 in a loop under the 1 kW cap; 16386 rows over 32 of these
+// experts 264 us by itself (floor 174) and 298 in a loop, with a row list to pack 277 and 332: the
+// tensor cores wait for the one accumulator at the end of each tile.  With f32 scales 397 and 444,
+// with a list 417 and 461: a worker's load of products, its wait and its additions follow one
+// another, neither the tensor pipe (36 %) nor the issue slots (35 %) are full.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -428,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<E8, NT>::THREAD
                         tma_gather4(dst + ABYTES + lane * 512, &p.tmA[0], ks * 128, make_int4(src[0], src[1], src[2], src[3]), fb);
                 } else if (lane < 4 && mine & 128 >> lane) {
                     // a sum of boxes, one a lane: a copy costs the TMA unit about as much whatever its
-                    // height (boxes of 16 rows alone: 2091 against 3050 TFLOP/s for one expert of
+                    // height (boxes of 16 rows alone took 1.46 times as long for one expert of
                     // 16384 rows, 4096 x 4096)
                     const int at = mine & ~(0xff >> lane);
                     tma_load2(dst + ABYTES + at * 128, &p.tmA[lane], ks * 128, t.r0 + half * rank + at, fb);

@@ -60,7 +60,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 // between the sum of squares and the output, and reads every input once.  A block of 128
 // columns is 16 neighbouring lanes.
 // Bound by HBM: 16384 x 4096 with residual and both outputs, 604 MB, takes 94 to 102 us, 6 TB/s
-// (one CTA per row: 114 us; the next row in registers: 102 us, and 4.1 TB/s at D = 8192).
+// (one CTA per row: 114 us; the next row in registers: 102 us, and 4.1 TB/s at D = 8192).  By
+// instructions where q is the only output: 203 MB without residual take 60 us, 3.4 TB/s (e8m0
+// scales 55 us, 3.7).
 // ---------------------------------------------------------------------------
 struct NormArgs {
     const uint4 *x, *res;
@@ -247,9 +249,9 @@ __global__ void __launch_bounds__(NORM_THREADS, CH == 4 ? 1 : 2) k_rms_norm_quan
 // sqrt(softplus) are screened in 32 bits first (route32); rows whose choice 32 bits
 // cannot settle, and softmax, take the 64-bit path (route64).  The chosen experts'
 // weights are in 64 bits on both.
-// Bound by instructions (about 1300 a token with 8 groups; the logits' bytes would take 1.4 us):
-// 8191 x 256, 8 groups, k = 8 takes 17 us.  All in 64 bits took 43, whole rows sent to route64
-// for one close call 28.
+// Bound by instructions (1461 a token with 8 groups; the logits' bytes would take 1.4 us): 8191 x
+// 256, k = 8, takes 16.3 us with 8 groups, 11.4 without; softmax, all in 64 bits, 24 us.  Sigmoid
+// and 8 groups all in 64 bits took 43, with whole rows sent to route64 for one close call 28.
 // ---------------------------------------------------------------------------
 constexpr int ROUTE_MAX_E = 512, ROUTE_MAX_K = 16, ROUTE_MAX_G = 32;
 constexpr int ROUTE_WARPS = 4;
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(32 * DISP_WARPS) k_dispatch_place(const __grid
 // in ascending row order (ascending expert, the layer's own order), in 32 bits.
 // A slot outside [0, R) adds nothing.  One CTA per token and 2048 columns, 8
 // columns per thread; the token's slots are sorted once per CTA.
-// Bound by HBM: 8192 tokens x 8 rows of 4096 with the shared rows, 671 MB, take 104 us,
+// Bound by HBM: 8192 tokens x 8 rows of 4096 with the shared rows, 671 MB, take 104 to 107 us,
 // 6.4 TB/s (one row's load at a time: 117 us; eight, with fewer CTAs on an SM: 112 us).
 // ---------------------------------------------------------------------------
 constexpr int COMB_MAX_K = 16;
