@@ -71,3 +71,12 @@ def test_an_entry_module_that_does_not_compile_is_an_error(entry, monkeypatch):
     entry.write_text("#error no\n")
     with pytest.raises(RuntimeError, match="failed"):
         _build.main(["_build"])
+
+
+def test_a_package_without_its_sources_loads_the_module_it_came_with(entry, monkeypatch):
+    """Copied with its built libraries alone: torch and Python still have to be those it was built for."""
+    os.remove(entry)
+    assert _build.ext_current()
+    assert L.load_ext(build_if_missing=False)
+    monkeypatch.setattr("torch.__version__", "1.0.0")
+    assert not _build.ext_current()

@@ -60,26 +60,32 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in deps())
 
 
-def ext_key() -> str:
-    """What the Python entry module is compiled from and against: its sources, torch, and the interpreter's ABI."""
+def ext_key():
+    """What the Python entry module is compiled against (torch, the interpreter's ABI) and from (its sources; empty in
+    a package without them), a line each."""
     import sysconfig
 
     import torch
 
-    key = hashlib.sha256(f"{torch.__version__} {sysconfig.get_config_var('SOABI')}".encode())
+    against = f"{torch.__version__} {sysconfig.get_config_var('SOABI')}"
+    if not all(os.path.exists(p) for p in ext_deps()):
+        return against, ""
+    source = hashlib.sha256()
     for p in ext_deps():
         with open(p, "rb") as f:
-            key.update(f.read())
-    return key.hexdigest()
+            source.update(f.read())
+    return against, source.hexdigest()
 
 
 def ext_current() -> bool:
-    """Whether the module in place is of this source, torch and interpreter (by the key written beside it)."""
+    """Whether the module in place is of this torch, interpreter and source (by the key written beside it)."""
     try:
         with open(EXT_KEY) as f:
-            return os.path.exists(EXT) and f.read() == ext_key()
+            has = f.read().split("\n")
     except FileNotFoundError:
         return False
+    against, source = ext_key()
+    return os.path.exists(EXT) and has[0] == against and (not source or has[1:] == [source])
 
 
 def _run(cmd, target, verbose):
@@ -120,7 +126,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     _run([cxx(), *flags, EXT_SRC, "-o", None, *libs], EXT, verbose)
     tmp = EXT_KEY + f".tmp{os.getpid()}"
     with open(tmp, "w") as f:
-        f.write(key)
+        f.write("\n".join(key))
     os.replace(tmp, EXT_KEY)
     return EXT
 
